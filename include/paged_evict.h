@@ -111,10 +111,16 @@ enum {
   PE_DIAG_SCORE_ROW_FULL = 2,     /* pe_evict_select_compact: a sequence's score row already
                                      held score_table_width entries; the new block's score was
                                      not appended                                              */
-  PE_DIAG_TABLE_STATE_MISMATCH = 4 /* pe_table_state_advance: the step's token does not fall into
+  PE_DIAG_TABLE_STATE_MISMATCH = 4, /* pe_table_state_advance: the step's token does not fall into
                                      the last block of the device-resident row (host and device
                                      counters disagree, or the row is full); the token's slot
                                      was reported as -1 (not cached)                           */
+  PE_DIAG_BLOCK_ID = 8,           /* the 8-bit and windowed calls: a block table names a block
+                                     outside [0, num_blocks); its tokens were not written, or
+                                     not attended                                              */
+  PE_DIAG_APPEND_MISMATCH = 16    /* pe_reshape_and_cache_8bit / pe_decode_step_8bit: cu_q,
+                                     seq_lens, the number of rows and the width of the tables do
+                                     not fit together; nothing of that sequence was written    */
 };
 int pe_device_diagnostics(unsigned int* flags_out, int reset);
 
@@ -652,6 +658,90 @@ int pe_copy_blocks(void* const* key_cache_ptrs, void* const* value_cache_ptrs,
                    int64_t numel_per_block, int dtype, void* stream);
 int pe_swap_blocks(const void* src, void* dst, const int64_t* block_mapping_host,
                    int64_t num_pairs, int64_t block_bytes, int kind, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Prefill attention with a sliding window and sink tokens: pe_prefill_causal whose query i attends
+ * kv rows j <= min(i, Lkv-1) with sliding_window == 0, or j > i - sliding_window, or j < num_sinks; a
+ * query that sees no row gets zeros.  bf16 / f16, head sizes 32, 64, 80, 96, 112, 120, 128, 192,
+ * 256, scale > 0.  max_q_len sizes the grid: rows of a request past it are not computed.  A NaN or
+ * an infinity in k or v reaches the queries that see its row, no other (such a tile costs much
+ * more time).
+ * ---------------------------------------------------------------------------------- */
+int pe_prefill_window(void* out, const void* q, const void* k, const void* v, const int32_t* cu_q,
+                      const int32_t* cu_kv, int num_seqs, int max_q_len, int num_heads,
+                      int num_kv_heads, int head_size, int64_t q_stride, int64_t k_stride,
+                      int64_t v_stride, int64_t out_stride, float scale, int sliding_window,
+                      int num_sinks, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * 8-bit paged cache.  Element = code * scale; codes e4m3 (largest value 448) or int8 (-127 ..
+ * 127); one f32 scale per (block, KV head) of K and of V.
+ *   key_cache   [num_blocks, num_kv_heads, head_size/16, block_size, 16]  codes
+ *   value_cache [num_blocks, num_kv_heads, head_size, block_size]         codes
+ *   kv_scales   f32 [num_blocks, num_kv_heads, 2]                         (K, V), contiguous
+ * (the layouts of the 16-bit cache with x = 16; strides in elements = bytes).  Head sizes 32, 64,
+ * 80, 96, 112, 128, 192, 256; block sizes 8, 16, 32; rows (query, key, value, out) in bf16 or f16.
+ * ---------------------------------------------------------------------------------- */
+typedef enum { PE_KV_SAME = 0, PE_KV_FP8_E4M3 = 1, PE_KV_INT8 = 2 } pe_kv_format;
+
+/* Appends rows to sequences of an 8-bit cache.  Sequence s takes rows cu_q[s] .. cu_q[s+1]-1 of
+ * key/value [num_tokens, num_kv_heads, head_size] (cu_q == NULL: row s, the rows of a decode step)
+ * at positions seq_lens[s] - rows .. seq_lens[s] - 1, i.e. seq_lens counts them already; a sequence
+ * with no rows or with length 0 is skipped.  max_q_len sizes the grid.
+ *   scale   s = max(s_old, 2^ceil(log2(max |x| / FMAX))) over the block's new rows (FMAX 448 or 127;
+ *           at least 2^-100; 0 while all is 0), s_old = 0 when the call writes offset 0 of the block:
+ *           a block begins anew there, whatever it held
+ *   codes   rn(x / s), to nearest even; where s grew, the block's older codes become
+ *           rn(code * s_old / s)
+ * x / s is exact (powers of two).  The scale is taken from finite elements; infinities become the
+ * largest code, NaN stays NaN (e4m3) or becomes 0 (int8).  Slots behind a sequence's last row are
+ * left as they are.  Two sequences must not append to one block. */
+int pe_reshape_and_cache_8bit(const void* key, const void* value, void* key_cache, void* value_cache,
+                              float* kv_scales, const int32_t* block_tables, const int32_t* seq_lens,
+                              const int32_t* cu_q, int num_seqs, int64_t num_tokens, int max_q_len,
+                              int64_t key_stride, int64_t value_stride, int num_kv_heads,
+                              int head_size, int block_size, int64_t num_blocks,
+                              int max_num_blocks_per_seq, int64_t kv_block_stride,
+                              int64_t kv_head_stride, int dtype, int kv_format, void* stream);
+
+/* Decode attention over an 8-bit cache, and over a 16-bit cache through a window.  The query of
+ * sequence s stands at position seq_lens[s] - 1 and sees the keys j < seq_lens[s] with
+ * sliding_window == 0, or j >= seq_lens[s] - sliding_window, or j < num_sinks; blocks that hold no
+ * such key are not read.  out [num_seqs, num_heads, head_size] dense; nothing visible: zeros.
+ * Any number of query heads per KV head.  Scales may be any finite f32 >= 0.
+ *   workspace  device scratch of at least pe_paged_window_workspace_bytes(...) bytes, NULL when that
+ *              is 0.  Calls that overlap on one workspace race on it. */
+int64_t pe_paged_window_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                                        int max_seq_len, int sliding_window, int num_sinks,
+                                        int kv_format);
+int pe_paged_decode_window(void* out, const void* query, const void* key_cache,
+                           const void* value_cache, const int32_t* block_tables,
+                           const int32_t* seq_lens, int num_seqs, int num_heads, int num_kv_heads,
+                           int head_size, int block_size, int64_t num_blocks,
+                           int max_num_blocks_per_seq, int64_t q_stride, int64_t kv_block_stride,
+                           int64_t kv_head_stride, float scale, int max_seq_len, int sliding_window,
+                           int num_sinks, int dtype, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+int pe_paged_decode_8bit(void* out, const void* query, const void* key_cache,
+                         const void* value_cache, const float* kv_scales,
+                         const int32_t* block_tables, const int32_t* seq_lens, int num_seqs,
+                         int num_heads, int num_kv_heads, int head_size, int block_size,
+                         int64_t num_blocks, int max_num_blocks_per_seq, int64_t q_stride,
+                         int64_t kv_block_stride, int64_t kv_head_stride, float scale,
+                         int max_seq_len, int sliding_window, int num_sinks, int dtype,
+                         int kv_format, void* workspace, int64_t workspace_bytes, void* stream);
+/* One decode layer over an 8-bit cache: pe_reshape_and_cache_8bit of one row per sequence
+ * (new_key / new_value [num_seqs, num_kv_heads, head_size]), then pe_paged_decode_8bit, which sees
+ * that row as the cache holds it. */
+int pe_decode_step_8bit(void* out, const void* query, const void* new_key, const void* new_value,
+                        void* key_cache, void* value_cache, float* kv_scales,
+                        const int32_t* block_tables, const int32_t* seq_lens, int num_seqs,
+                        int num_heads, int num_kv_heads, int head_size, int block_size,
+                        int64_t num_blocks, int max_num_blocks_per_seq, int64_t q_stride,
+                        int64_t new_k_stride, int64_t new_v_stride, int64_t kv_block_stride,
+                        int64_t kv_head_stride, float scale, int max_seq_len, int sliding_window,
+                        int num_sinks, int dtype, int kv_format, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,6 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpaged_evict.so")
 
 PE_F32, PE_F16, PE_BF16 = 0, 1, 2
+PE_KV_SAME, PE_KV_FP8_E4M3, PE_KV_INT8 = 0, 1, 2
 
 # name -> (restype, argtypes); must list every symbol include/paged_evict.h declares
 SIGNATURES = {
@@ -107,6 +108,28 @@ SIGNATURES = {
     "pe_copy_blocks": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int,
                                c_void_p]),
     "pe_swap_blocks": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p]),
+    "pe_prefill_window": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                  c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64,
+                                  c_float, c_int, c_int, c_int, c_void_p]),
+    "pe_reshape_and_cache_8bit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int,
+                                          c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int,
+                                          c_int64, c_int64, c_int, c_int, c_void_p]),
+    "pe_paged_window_workspace_bytes": (c_int64, [c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                                  c_int]),
+    "pe_paged_decode_window": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int64,
+                                       c_int64, c_int64, c_float, c_int, c_int, c_int, c_int,
+                                       c_void_p, c_int64, c_void_p]),
+    "pe_paged_decode_8bit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_int,
+                                     c_int64, c_int64, c_int64, c_float, c_int, c_int, c_int, c_int,
+                                     c_int, c_void_p, c_int64, c_void_p]),
+    "pe_decode_step_8bit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                    c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                    c_float, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64,
+                                    c_void_p]),
 }
 
 _lib = None

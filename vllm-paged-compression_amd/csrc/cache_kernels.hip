@@ -258,11 +258,13 @@ void pe_reload_env(void) { pe::g_env_generation.fetch_add(1, std::memory_order_r
 
 int pe_device_diagnostics(unsigned int* flags_out, int reset) {
   PE_REQUIRE(flags_out != nullptr, PE_ERR_INVALID_ARG, "device_diagnostics: null pointer");
-  unsigned int a = 0, b = 0, c = 0;
+  unsigned int a = 0, b = 0, c = 0, d = 0, e = 0;
   if (int rc = pe::decode_diag_fetch(&a, reset)) return rc;
   if (int rc = pe::evict_diag_fetch(&b, reset)) return rc;
   if (int rc = pe::state_diag_fetch(&c, reset)) return rc;
-  *flags_out = a | b | c;
+  if (int rc = pe::window_diag_fetch(&d, reset)) return rc;
+  if (int rc = pe::cache8_diag_fetch(&e, reset)) return rc;
+  *flags_out = a | b | c | d | e;
   return PE_OK;
 }
 

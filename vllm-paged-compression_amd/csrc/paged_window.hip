@@ -1,0 +1,152 @@
+// Entry points of the windowed and the 8-bit decode attention (kernel: paged_window_kernel.h)
+//   pe_paged_decode_window   16-bit cache, sliding window + sink tokens
+//   pe_paged_decode_8bit     8-bit cache, with or without a window
+//   pe_decode_step_8bit      KV write of the step's token + the attention
+#include "paged_window_kernel.h"
+
+namespace pe {
+
+int launch_window_16(const WinArgs& a, int head_size, int block_size, int dtype, dim3 grid, hipStream_t st);
+int launch_window_fp8(const WinArgs& a, int head_size, int block_size, int dtype, dim3 grid, hipStream_t st);
+int launch_window_int8(const WinArgs& a, int head_size, int block_size, int dtype, dim3 grid, hipStream_t st);
+int window_16_diag_fetch(unsigned int* out, int reset);
+int window_fp8_diag_fetch(unsigned int* out, int reset);
+int window_int8_diag_fetch(unsigned int* out, int reset);
+
+int window_diag_fetch(unsigned int* out, int reset) {
+  unsigned int a = 0, b = 0, c = 0;
+  if (int rc = window_16_diag_fetch(&a, reset)) return rc;
+  if (int rc = window_fp8_diag_fetch(&b, reset)) return rc;
+  if (int rc = window_int8_diag_fetch(&c, reset)) return rc;
+  *out = a | b | c;
+  return PE_OK;
+}
+
+static int window_splits(int num_seqs, int num_heads, int num_kv_heads, int max_seq_len, int window,
+                         int sinks, int kv_format) {
+  return 1;
+}
+
+static int check_window(const char* who, int window, int sinks) {
+  PE_REQUIRE(window >= 0 && sinks >= 0, PE_ERR_INVALID_ARG,
+             "%s: sliding_window %d and num_sinks %d must not be negative", who, window, sinks);
+  return PE_OK;
+}
+
+static int window_decode(const char* who, void* out, const void* query, const void* key_cache,
+                         const void* value_cache, const float* kv_scales, const int32_t* block_tables,
+                         const int32_t* seq_lens, int num_seqs, int num_heads, int num_kv_heads,
+                         int head_size, int block_size, int64_t num_blocks, int table_width,
+                         int64_t q_stride, int64_t kv_block_stride, int64_t kv_head_stride, float scale,
+                         int max_seq_len, int window, int sinks, int dtype, int kv_format,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+  PE_REQUIRE(out && query && key_cache && value_cache && block_tables && seq_lens, PE_ERR_INVALID_ARG,
+             "%s: null pointer", who);
+  PE_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0, PE_ERR_INVALID_ARG,
+             "%s: num_heads %d must be a positive multiple of num_kv_heads %d", who, num_heads, num_kv_heads);
+  PE_REQUIRE(max_seq_len >= 0, PE_ERR_INVALID_ARG, "%s: negative max_seq_len", who);
+  PE_REQUIRE(q_stride % 8 == 0 && (uintptr_t)query % 16 == 0, PE_ERR_INVALID_ARG,
+             "%s: query rows must be 16-byte aligned", who);
+  const int gqa = num_heads / num_kv_heads, groups = (gqa + 15) / 16;
+  PE_REQUIRE(num_seqs <= 65535 && (int64_t)num_kv_heads * groups <= 65535, PE_ERR_UNSUPPORTED,
+             "%s: grid too large", who);
+  const int splits = window_splits(num_seqs, num_heads, num_kv_heads, max_seq_len, window, sinks, kv_format);
+  if (splits > 1) {
+    const int64_t need = (int64_t)splits * num_seqs * num_heads * win_ws_stride(head_size) * 4;
+    PE_REQUIRE(workspace && workspace_bytes >= need, PE_ERR_WORKSPACE, "%s needs %lld workspace bytes, got %lld",
+               who, (long long)need, (long long)workspace_bytes);
+  }
+  const WinArgs a{out, (float*)workspace, query, key_cache, value_cache, kv_scales, block_tables, seq_lens,
+                  num_heads, num_kv_heads, table_width, window, sinks, splits, groups, num_blocks, q_stride,
+                  kv_block_stride, kv_head_stride, scale * 1.4426950408889634f};
+  const dim3 grid((unsigned)splits, (unsigned)(num_kv_heads * groups), (unsigned)num_seqs);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int rc;
+  if (kv_format == PE_KV_FP8_E4M3) rc = launch_window_fp8(a, head_size, block_size, dtype, grid, st);
+  else if (kv_format == PE_KV_INT8) rc = launch_window_int8(a, head_size, block_size, dtype, grid, st);
+  else rc = launch_window_16(a, head_size, block_size, dtype, grid, st);
+  if (rc) return rc;
+  return check_launch(who);
+}
+
+}  // namespace pe
+
+extern "C" {
+
+int64_t pe_paged_window_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                                        int max_seq_len, int sliding_window, int num_sinks, int kv_format) {
+  using namespace pe;
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0) return 0;
+  const int splits = window_splits(num_seqs, num_heads, num_kv_heads, max_seq_len, sliding_window, num_sinks, kv_format);
+  return splits <= 1 ? 0 : (int64_t)splits * num_seqs * num_heads * win_ws_stride(head_size) * 4;
+}
+
+int pe_paged_decode_window(void* out, const void* query, const void* key_cache, const void* value_cache,
+                           const int32_t* block_tables, const int32_t* seq_lens, int num_seqs,
+                           int num_heads, int num_kv_heads, int head_size, int block_size,
+                           int64_t num_blocks, int max_num_blocks_per_seq, int64_t q_stride,
+                           int64_t kv_block_stride, int64_t kv_head_stride, float scale,
+                           int max_seq_len, int sliding_window, int num_sinks, int dtype,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace pe;
+  const char* who = "paged_decode_window";
+  PE_REQUIRE(num_seqs >= 0, PE_ERR_INVALID_ARG, "%s: negative num_seqs", who);
+  if (num_seqs == 0) return PE_OK;
+  if (int rc = check_window(who, sliding_window, num_sinks)) return rc;
+  PE_REQUIRE(dtype == PE_BF16 || dtype == PE_F16, PE_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or f16)", who, dtype);
+  PE_REQUIRE(num_blocks > 0 && max_num_blocks_per_seq > 0, PE_ERR_INVALID_ARG, "%s: bad sizes", who);
+  PE_REQUIRE((int64_t)max_num_blocks_per_seq * block_size <= (1 << 30), PE_ERR_UNSUPPORTED,
+             "%s: block tables of %d blocks address more than 2^30 tokens", who, max_num_blocks_per_seq);
+  PE_REQUIRE(kv_block_stride % 8 == 0 && kv_head_stride % 8 == 0 &&
+                 ((uintptr_t)key_cache | (uintptr_t)value_cache) % 16 == 0,
+             PE_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", who);
+  return window_decode(who, out, query, key_cache, value_cache, nullptr, block_tables, seq_lens, num_seqs,
+                       num_heads, num_kv_heads, head_size, block_size, num_blocks, max_num_blocks_per_seq,
+                       q_stride, kv_block_stride, kv_head_stride, scale, max_seq_len, sliding_window,
+                       num_sinks, dtype, PE_KV_SAME, workspace, workspace_bytes, stream);
+}
+
+int pe_paged_decode_8bit(void* out, const void* query, const void* key_cache, const void* value_cache,
+                         const float* kv_scales, const int32_t* block_tables, const int32_t* seq_lens,
+                         int num_seqs, int num_heads, int num_kv_heads, int head_size, int block_size,
+                         int64_t num_blocks, int max_num_blocks_per_seq, int64_t q_stride,
+                         int64_t kv_block_stride, int64_t kv_head_stride, float scale, int max_seq_len,
+                         int sliding_window, int num_sinks, int dtype, int kv_format, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  using namespace pe;
+  const char* who = "paged_decode_8bit";
+  PE_REQUIRE(num_seqs >= 0, PE_ERR_INVALID_ARG, "%s: negative num_seqs", who);
+  if (num_seqs == 0) return PE_OK;
+  PE_REQUIRE(kv_scales, PE_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (int rc = check_window(who, sliding_window, num_sinks)) return rc;
+  if (int rc = check_cache8(who, key_cache, value_cache, kv_scales, num_kv_heads, head_size, block_size,
+                            num_blocks, max_num_blocks_per_seq, kv_block_stride, kv_head_stride, dtype, kv_format))
+    return rc;
+  return window_decode(who, out, query, key_cache, value_cache, kv_scales, block_tables, seq_lens, num_seqs,
+                       num_heads, num_kv_heads, head_size, block_size, num_blocks, max_num_blocks_per_seq,
+                       q_stride, kv_block_stride, kv_head_stride, scale, max_seq_len, sliding_window,
+                       num_sinks, dtype, kv_format, workspace, workspace_bytes, stream);
+}
+
+int pe_decode_step_8bit(void* out, const void* query, const void* new_key, const void* new_value,
+                        void* key_cache, void* value_cache, float* kv_scales, const int32_t* block_tables,
+                        const int32_t* seq_lens, int num_seqs, int num_heads, int num_kv_heads,
+                        int head_size, int block_size, int64_t num_blocks, int max_num_blocks_per_seq,
+                        int64_t q_stride, int64_t new_k_stride, int64_t new_v_stride,
+                        int64_t kv_block_stride, int64_t kv_head_stride, float scale, int max_seq_len,
+                        int sliding_window, int num_sinks, int dtype, int kv_format, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  if (int rc = pe_reshape_and_cache_8bit(new_key, new_value, key_cache, value_cache, kv_scales, block_tables,
+                                         seq_lens, nullptr, num_seqs, num_seqs, 1, new_k_stride, new_v_stride,
+                                         num_kv_heads, head_size, block_size, num_blocks,
+                                         max_num_blocks_per_seq, kv_block_stride, kv_head_stride, dtype,
+                                         kv_format, stream))
+    return rc;
+  return pe_paged_decode_8bit(out, query, key_cache, value_cache, kv_scales, block_tables, seq_lens, num_seqs,
+                              num_heads, num_kv_heads, head_size, block_size, num_blocks,
+                              max_num_blocks_per_seq, q_stride, kv_block_stride, kv_head_stride, scale,
+                              max_seq_len, sliding_window, num_sinks, dtype, kv_format, workspace,
+                              workspace_bytes, stream);
+}
+
+}  // extern "C"
