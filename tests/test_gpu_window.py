@@ -98,6 +98,24 @@ def test_prefill_window_longer_prompts(ops):
         plain.assert_within(got, ref, bound, f"window {window}, sinks {sinks}")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,H,D", [(32, 8, 128), (40, 40, 96), (48, 8, 112)])
+@pytest.mark.parametrize("window,sinks", [(64, 4), (250, 38), (251, 38), (400, 0), (0, 0)])
+def test_prefill_window_launches_that_fill_the_chip(ops, dtype, Hq, H, D, window, sinks):
+    """More than 256 workgroups: the shapes for rows that see few keys and for rows that see many, with 4, 1
+    and 2 query heads side by side in a workgroup."""
+    g = torch.Generator().manual_seed(Hq + D + window)
+    lens = [513, 300, 290]
+    T = sum(lens)
+    q, k, v = rows(g, T, Hq, D, dtype), rows(g, T, H, D, dtype), rows(g, T, H, D, dtype)
+    got = run_prefill(ops, q, k, v, lens, lens, window, sinks, D ** -0.5)
+    pick = [0, Hq // H, Hq - 1]                        # the reference of every head would take minutes
+    ref, bound = prefill_reference(q[:, pick], k[:, [p * H // Hq for p in pick]], v[:, [p * H // Hq for p in pick]],
+                                   lens, lens, window, sinks, D ** -0.5)
+    plain.assert_within(got[:, pick], ref, bound, f"window {window}, sinks {sinks}")
+    assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("sinks", [0, 3])
 def test_prefill_window_fewer_or_more_kv_rows(ops, sinks):
     """A pruned prompt (rows whose window lies past the last kv row see the sinks or nothing: zeros), more
@@ -122,9 +140,13 @@ def test_prefill_window_equals_causal_without_a_window(ops):
     lens = [300, 41]
     q, k, v = (rows(g, 341, h, 128, torch.bfloat16).cuda() for h in (8, 2, 2))
     cu = torch.tensor([0, 300, 341], dtype=torch.int32).cuda()
-    a = ops.prefill_causal(q, k, v, cu, cu, 300, 128 ** -0.5)
-    for window, sinks in ((0, 0), (300, 0), (2 ** 31 - 1, 2 ** 31 - 1)):
-        assert torch.equal(a, ops.prefill_window(q, k, v, cu, cu, 300, 128 ** -0.5, window, sinks))
+    ref, bound = prefill_reference(q.cpu(), k.cpu(), v.cpu(), [300, 41], [300, 41], 0, 0, 128 ** -0.5)
+    plain.assert_within(ops.prefill_causal(q, k, v, cu, cu, 300, 128 ** -0.5), ref, bound)
+    a = ops.prefill_window(q, k, v, cu, cu, 300, 128 ** -0.5, 0, 0)
+    for window, sinks in ((300, 0), (2 ** 31 - 1, 2 ** 31 - 1), (17, 300)):
+        b = ops.prefill_window(q, k, v, cu, cu, 300, 128 ** -0.5, window, sinks)
+        plain.assert_within(b, ref, bound, f"window {window}, sinks {sinks}")
+    plain.assert_within(a, ref, bound)
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])

@@ -75,22 +75,24 @@ __device__ __forceinline__ float max_xor_16_32(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-template <typename T, int D, int NR, int WAVES, int WPE, bool WIN = false>
+template <typename T, int D, int NR, int WAVES, int WPE, bool WIN = false, int BN = PF_BN>
 __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ k,
     const T* __restrict__ v, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_kv,
     int num_heads, int num_kv_heads, int head_size, int64_t q_stride, int64_t k_stride,
-    int64_t v_stride, int64_t out_stride, float scale_log2e, int window, int sinks) {
-  // window, sinks: WIN only
+    int64_t v_stride, int64_t out_stride, float scale_log2e, int window, int sinks,
+    int heads_per_wg) {
+  // window, sinks, heads_per_wg: WIN only
   using TR = Traits<T>;
   using vec8 = typename TR::vec8;
   constexpr int KS = D / 32;
   constexpr int DT = D / 16;
+  constexpr int NS = BN / 16;                       // 16-key groups of a tile
   constexpr int CPR = D / 8;                        // 16-byte chunks per row
-  constexpr int TILE_BYTES = PF_BN * D * 2;         // one K or V tile
+  constexpr int TILE_BYTES = BN * D * 2;         // one K or V tile
   constexpr int WROWS = 16 * NR;                    // query rows per wave
   constexpr int BM = WROWS * WAVES;                 // query rows per workgroup
-  static_assert(BM % PF_BN == 0 && BM * D * 2 <= 4 * TILE_BYTES, "tile shape");
+  static_assert(BM % BN == 0 && BM * D * 2 <= 4 * TILE_BYTES, "tile shape");
 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // [buf][K|V][tile]
@@ -102,7 +104,11 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   // workgroup ids go to consecutive XCDs; the (head, request) plane is re-enumerated so that all
   // query heads of one (request, KV head) - which read the same K/V - get ids that are equal
   // modulo 8 and share one XCD's L2 (needs num_kv_heads * num_requests to be a multiple of 8).
-  const int gqa = num_heads / num_kv_heads;
+  // WIN: the waves of a workgroup take the same query rows of heads_per_wg query heads of one KV head
+  // (and, where there are more waves, further rows), so that they see nearly the same keys: a
+  // workgroup streams window + rows / heads_per_wg keys instead of window + rows.
+  const int hpw = WIN ? heads_per_wg : 1;
+  const int gqa = num_heads / num_kv_heads / hpw;  // workgroups side by side on a KV head
   const int lid = (int)blockIdx.x + (int)gridDim.x * (int)blockIdx.y;
   const int n_groups = num_kv_heads * (int)gridDim.y;
   int grp, hg;
@@ -115,18 +121,19 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   }
   const int seq = grp / num_kv_heads;
   const int kvh = grp % num_kv_heads;
-  const int head = kvh * gqa + hg;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int head = WIN ? (kvh * gqa + hg) * hpw + wave % hpw : kvh * gqa + hg;
+  const int bm = WIN ? BM / hpw : BM;  // query rows per workgroup and head
   const int q0 = cu_q[seq], lq = cu_q[seq + 1] - q0;
   const int kv0 = cu_kv[seq], lkv = cu_kv[seq + 1] - kv0;
   const int qt = (int)gridDim.z - 1 - (int)blockIdx.z;
-  const int m0 = qt * BM;
+  const int m0 = qt * bm;
   if (m0 >= lq) return;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
-  const int wrow0 = m0 + wave * WROWS;  // first query row of this wave
+  const int wrow0 = m0 + (WIN ? wave / hpw : wave) * WROWS;  // first query row of this wave
   const int hchunks = head_size >> 3;   // 16-byte chunks of a head row that exist (<= CPR)
 
   // ---- Q fragments (B operand): lane holds Q[row][32ks + 8g .. +8) for its row tiles ----
@@ -162,14 +169,14 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     for (int dt = 0; dt < DT; ++dt) acc[dt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int kv_end = min(lkv, m0 + BM);  // rows past the last query row are never attended
-  const int n_tiles = (kv_end + PF_BN - 1) / PF_BN;
+  const int kv_end = min(lkv, m0 + bm);  // rows past the last query row are never attended
+  const int n_tiles = (kv_end + BN - 1) / BN;
   // WIN: the tiles visited are [0, ns) (sinks) and [tw, n_tiles) (windows of the workgroup's rows)
   int ns = 0, tw = 0;
   if constexpr (WIN) {
     const int lo = window > 0 ? max(0, m0 - window + 1) : 0;
-    tw = lo / PF_BN;
-    ns = min((min(sinks, kv_end) + PF_BN - 1) / PF_BN, tw);
+    tw = lo / BN;
+    ns = min((min(sinks, kv_end) + BN - 1) / BN, tw);
   }
 
   // Staging: K/V tiles go global -> LDS directly (global_load_lds_dwordx4, no registers, no
@@ -183,8 +190,8 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   // reads of the tile.
   constexpr int RPI = 64 / CPR;            // tile rows per wave-instruction
   constexpr int RSTEP = WAVES * RPI;       // rows between a wave's consecutive instructions
-  constexpr int NINST = PF_BN / RSTEP;     // instructions per wave per operand tile
-  static_assert(RSTEP % 16 == 0 && NINST >= 1 && NINST * RSTEP == PF_BN, "staging shape");
+  constexpr int NINST = BN / RSTEP;     // instructions per wave per operand tile
+  static_assert(RSTEP % 16 == 0 && NINST >= 1 && NINST * RSTEP == BN, "staging shape");
   const int lrow = wave * RPI + lane / CPR;  // row within a RSTEP group
   const int lslot = lane % CPR;
   const char* k_seq = reinterpret_cast<const char*>(k + (int64_t)kv0 * k_stride + (int64_t)kvh * head_size);
@@ -227,12 +234,12 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     }
   };
   auto stage = [&](int tile, int buf) {
-    const int t0 = tile * PF_BN;
+    const int t0 = tile * BN;
     const char* kb = k_seq + (int64_t)t0 * k_row_bytes;
     const char* vb = v_seq + (int64_t)t0 * v_row_bytes;
     const uint32_t kd = lds0 + (uint32_t)buf * (2u * TILE_BYTES);
     const uint32_t vd = kd + TILE_BYTES;
-    if (t0 + PF_BN <= lkv) {
+    if (t0 + BN <= lkv) {
       glds16(kb, k_lane_off, kd, std::true_type{});
       glds16(vb, v_lane_off, vd, std::false_type{});
 #pragma unroll
@@ -257,16 +264,41 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   };
   auto stage_wait = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
 
+  // O^T += V^T.P^T over 32 keys of a tile, and the row sums
+  // transposed read: lane i of each 16-lane group addresses row (4g + i/4), columns
+  // 16dt + 4*(i%4) .. +4 and receives column 16dt+i of the group's 4 rows
+  auto pv_step = [&](const char* vt, int k2, const vec8 (&pf)[NR][NS / 2]) {
+    const int tq = c >> 2, tp = c & 3;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) acc_l[n] = TR::mfma16(ones, pf[n][k2], acc_l[n]);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int row_lo = (2 * k2) * 16 + 4 * g + tq;
+      const int row_hi = row_lo + 16;
+      const int ch = 2 * dt + (tp >> 1);
+      const int sub8 = (tp & 1) * 8;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(vt + swz_off_v<D>(row_lo, ch) + sub8));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(vt + swz_off_v<D>(row_hi, ch) + sub8));
+      typedef __attribute__((ext_vector_type(8))) short s16x8;
+      const s16x8 both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      const vec8 vf = __builtin_bit_cast(vec8, both);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) acc[dt][n] = TR::mfma16(vf, pf[n][k2], acc[dt][n]);
+    }
+  };
+
   auto compute = [&](int tile, int buf, auto masked_tag) {
     constexpr bool MASKED = decltype(masked_tag)::value;
-    const int n0 = tile * PF_BN;
+    const int n0 = tile * BN;
     const char* kt = k_tile(buf);
     const char* vt = v_tile(buf);
     // ---- S^T = K.Q^T ---------------------------------------------------------------
     // The K fragments of row group sub+1 are requested before the MFMAs of group sub are issued
     // (the scheduling fences keep that order), so that an MFMA waits for reads issued a whole
     // group earlier instead of for the read right in front of it.
-    f32x4 s[4][NR];
+    f32x4 s[NS][NR];
     vec8 kf[2][KS];
     auto load_k = [&](int sub, vec8* dst) {
 #pragma unroll
@@ -276,8 +308,8 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     };
     load_k(0, kf[0]);
 #pragma unroll
-    for (int sub = 0; sub < 4; ++sub) {
-      if (sub + 1 < 4) load_k(sub + 1, kf[(sub + 1) & 1]);
+    for (int sub = 0; sub < NS; ++sub) {
+      if (sub + 1 < NS) load_k(sub + 1, kf[(sub + 1) & 1]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < NR; ++n) s[sub][n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -290,36 +322,21 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     }
     // ---- mask, online softmax (the scale rides in the exponent's fma; maxima are kept in
     //      scaled log2 units, which needs scale > 0 - the launcher guarantees it) ----------
-    vec8 pf[NR][2];
+    vec8 pf[NR][NS / 2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       float mx = PF_NEG;
-      if constexpr (MASKED && WIN) {
-        // a row's first tiles may hide all their keys from it: -inf makes their weights 0 whatever
-        // the (finite) reference point is
-        const int qrow = wrow0 + n * 16 + c;
-        const int last = min(qrow, lkv - 1) - n0 - 4 * g;
-        const int first = (window > 0 ? qrow - window + 1 : 0) - n0 - 4 * g;
-        const int sink = sinks - n0 - 4 * g;
-        mx = -INFINITY;
-#pragma unroll
-        for (int sub = 0; sub < 4; ++sub)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = sub * 16 + r;
-            s[sub][n][r] = (j <= last && (j >= first || j < sink)) ? s[sub][n][r] : -INFINITY;
-          }
-      } else if constexpr (MASKED) {
+      if constexpr (MASKED) {
         const int qrow = wrow0 + n * 16 + c;
         const int limit = min(qrow, lkv - 1) - n0 - 4 * g;  // last attended (sub*16 + r)
 #pragma unroll
-        for (int sub = 0; sub < 4; ++sub)
+        for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             s[sub][n][r] = (sub * 16 + r <= limit) ? s[sub][n][r] : PF_NEG;
       }
 #pragma unroll
-      for (int sub = 0; sub < 4; ++sub)
+      for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[sub][n][r]);
       mx = max_xor_16_32(mx);
@@ -338,7 +355,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
       }
       const float m_new = m_run[n];
 #pragma unroll
-      for (int sub = 0; sub < 4; ++sub) {
+      for (int sub = 0; sub < NS; ++sub) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], scale_log2e, -m_new));
@@ -346,31 +363,83 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
         }
       }
     }
-    // ---- O^T += V^T.P^T ------------------------------------------------------------------
-    // transposed read: lane i of each 16-lane group addresses row (4g + i/4), columns
-    // 16dt + 4*(i%4) .. +4 and receives column 16dt+i of the group's 4 rows
-    const int tq = c >> 2, tp = c & 3;
 #pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2) {
+    for (int k2 = 0; k2 < NS / 2; ++k2) pv_step(vt, k2, pf);
+  };
+
+  // WIN: a tile that some of the wave's rows see only in part.  Row groups of 16 keys that no row of
+  // the wave sees are left out (a few sinks then cost a quarter of a tile).  Hidden scores become
+  // -inf, which makes their weights 0 whatever the (finite) reference point is: a row's first tiles
+  // may hide all their keys from it.
+  auto compute_part = [&](int tile, int buf) {
+    const int n0 = tile * BN;
+    const char* kt = k_tile(buf);
+    const char* vt = v_tile(buf);
+    const int row_last = wrow0 + WROWS - 1;
+    const int low = window > 0 ? wrow0 - window + 1 : 0;
+    const int high = min(row_last, lkv - 1);
+    bool on[NS];
 #pragma unroll
-      for (int n = 0; n < NR; ++n) acc_l[n] = TR::mfma16(ones, pf[n][k2], acc_l[n]);
+    for (int sub = 0; sub < NS; ++sub) {
+      const int k0 = n0 + sub * 16;
+      on[sub] = k0 <= high && (k0 + 15 >= low || k0 < sinks);
+    }
+    f32x4 s[NS][NR];
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const int row_lo = (2 * k2) * 16 + 4 * g + tq;
-        const int row_hi = row_lo + 16;
-        const int ch = 2 * dt + (tp >> 1);
-        const int sub8 = (tp & 1) * 8;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(vt + swz_off_v<D>(row_lo, ch) + sub8));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(vt + swz_off_v<D>(row_hi, ch) + sub8));
-        typedef __attribute__((ext_vector_type(8))) short s16x8;
-        const s16x8 both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        const vec8 vf = __builtin_bit_cast(vec8, both);
+    for (int sub = 0; sub < NS; ++sub) {
+      if (on[sub]) {
+        vec8 kf[KS];
 #pragma unroll
-        for (int n = 0; n < NR; ++n) acc[dt][n] = TR::mfma16(vf, pf[n][k2], acc[dt][n]);
+        for (int ks = 0; ks < KS; ++ks)
+          kf[ks] = __builtin_bit_cast(
+              vec8, *reinterpret_cast<const u32x4*>(kt + swz_off<D>(sub * 16 + c, 4 * ks + g)));
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          s[sub][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) s[sub][n] = TR::mfma16(kf[ks], qf[n][ks], s[sub][n]);
+          const int qrow = wrow0 + n * 16 + c;
+          const int last = min(qrow, lkv - 1) - n0 - 4 * g - sub * 16;
+          const int first = (window > 0 ? qrow - window + 1 : 0) - n0 - 4 * g - sub * 16;
+          const int sink = sinks - n0 - 4 * g - sub * 16;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[sub][n][r] = (r <= last && (r >= first || r < sink)) ? s[sub][n][r] : -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[sub][n] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       }
     }
+    vec8 pf[NR][NS / 2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub)
+        if (on[sub]) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[sub][n][r]);
+        }
+      const float m_tile = max_xor_16_32(mx) * scale_log2e;
+      if (__builtin_amdgcn_ballot_w64(m_tile > m_run[n] + PF_LAZY_LOG2) != 0) {  // wave-uniform
+        const float m_new = fmaxf(m_run[n], m_tile);
+        const float alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+        m_run[n] = m_new;
+        acc_l[n] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt][n] *= alpha;
+      }
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          pf[n][sub >> 1][(sub & 1) * 4 + r] =
+              on[sub] ? (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], scale_log2e, -m_run[n])) : (T)0.f;
+    }
+#pragma unroll
+    for (int k2 = 0; k2 < NS / 2; ++k2)
+      if (on[2 * k2] || on[2 * k2 + 1]) pv_step(vt, k2, pf);
   };
 
   // ---- main loop: tiles every wave attends in full first (no mask code), then the diagonal /
@@ -381,7 +450,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
       const int buf = tile & 1;
       if (tile + 1 < n_tiles) stage(tile + 1, buf ^ 1);
       // wave-uniform: skip a tile that is fully masked for all of this wave's rows
-      if (!MASKED || tile * PF_BN <= wrow0 + WROWS - 1) compute(tile, buf, masked_tag);
+      if (!MASKED || tile * BN <= wrow0 + WROWS - 1) compute(tile, buf, masked_tag);
       stage_wait();
       __syncthreads();
     }
@@ -401,18 +470,18 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
       for (int i = 0; i < count; ++i) {
         const int tile = tile_at(i), buf = i & 1;
         if (i + 1 < count) stage(tile_at(i + 1), buf ^ 1);
-        const int k0 = tile * PF_BN, k1 = k0 + PF_BN - 1;
+        const int k0 = tile * BN, k1 = k0 + BN - 1;
         // wave-uniform: some row sees some key / every row sees every key
         const bool some = k0 <= wrow1 && (window == 0 || k1 > wrow0 - window || k0 < sinks);
         const bool all = k1 <= wrow0 && k1 < lkv && (window == 0 || k0 > wrow1 - window || k1 < sinks);
         if (all) compute(tile, buf, std::false_type{});
-        else if (some) compute(tile, buf, std::true_type{});
+        else if (some) compute_part(tile, buf);
         stage_wait();
         __syncthreads();
       }
     }
   } else if (n_tiles > 0) {
-    const int n_full = min(min(m0, lkv) / PF_BN, n_tiles);
+    const int n_full = min(min(m0, lkv) / BN, n_tiles);
     stage(0, 0);
     // Retire the Q loads here: an empty asm that "rewrites" the fragments makes the compiler wait
     // for them before the loop instead of carrying them as pending into its wait-count

@@ -32,24 +32,42 @@ extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const 
   if (num_sinks > (1 << 30)) num_sinks = 1 << 30;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const float sl2 = scale * 1.4426950408889634f;
-#define PE_LAUNCH_PW(T, HS, NR, WAVES, WPE)                                                             \
+  // Tile shape: 16 x NR query rows per wave, 4 waves (8 at the 256 pitch), BN keys per tile.  The waves
+  // take the query heads of a KV head side by side (hpw of them).  Measured on MI355X (us per launch,
+  // 2 rows-tiles x 64 keys / 1 x 64 / 1 x 32; 32 query and 8 KV heads x 128, 4 sinks; window 0 = none):
+  //   8 x 1024 tokens, window 64: 58 / 63 / 44, 128: 58 / 69 / 52, 256: 67 / 81 / 65, 512: 80 / 100 / 86,
+  //   none: 89 / 110 / 99; 4 x 4096, window 64: 114 / 142 / 97, 256: 144 / 185 / 149, 1024: 289 / 368 / 338;
+  //   1 x 512, window 64: 12.0 / 8.7 / 8.7, none: 17.9 / 13.7 / 16.7;
+  //   12 heads x 64, 8 x 1024, window 64: 25 / 18 / 19, 256: 32 / 23 / 25, none: 33 / 28 / 34.
+  // So: head sizes up to 64, and launches that leave CUs idle, take the 1 x 64 shape (more, smaller
+  // workgroups; at 64 elements a key costs half the LDS reads); rows that see few
+  // keys the 1 x 32 shape, whose tiles waste less at the window's two ends; everything else 2 x 64,
+  // which reads each K/V fragment from LDS once for 32 rows.
+  const int gqa = num_heads / num_kv_heads;
+  const int64_t span = sliding_window > 0 ? (int64_t)sliding_window + num_sinks : max_q_len;
+  const int64_t wgs = (int64_t)num_seqs * num_heads * ((max_q_len + 127) / 128);  // of 2 x 64
+#define PE_LAUNCH_PW(T, HS, NR, WAVES, WPE, BN)                                                         \
   do {                                                                                                  \
-    const int bm = 16 * NR * WAVES;                                                                     \
-    dim3 grid((unsigned)num_heads, (unsigned)num_seqs, (unsigned)((max_q_len + bm - 1) / bm));          \
-    const size_t lds = 4 * (size_t)PF_BN * HS * 2;                                                      \
+    int hpw = WAVES;                                                                                    \
+    while (gqa % hpw) hpw /= 2;                                                                         \
+    const int bm = 16 * NR * WAVES / hpw;                                                               \
+    dim3 grid((unsigned)(num_heads / hpw), (unsigned)num_seqs, (unsigned)((max_q_len + bm - 1) / bm));  \
+    const size_t lds = 4 * (size_t)BN * HS * 2;                                                         \
     if (lds > 64 * 1024)                                                                                \
       (void)hipFuncSetAttribute(                                                                        \
-          reinterpret_cast<const void*>(&prefill_mfma_kernel<T, HS, NR, WAVES, WPE, true>),             \
+          reinterpret_cast<const void*>(&prefill_mfma_kernel<T, HS, NR, WAVES, WPE, true, BN>),         \
           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);                                        \
-    hipLaunchKernelGGL((prefill_mfma_kernel<T, HS, NR, WAVES, WPE, true>), grid, dim3(WAVES * 64), lds, \
-                       st, (T*)out, (const T*)q, (const T*)k, (const T*)v, cu_q, cu_kv, num_heads,      \
+    hipLaunchKernelGGL((prefill_mfma_kernel<T, HS, NR, WAVES, WPE, true, BN>), grid, dim3(WAVES * 64),  \
+                       lds, st, (T*)out, (const T*)q, (const T*)k, (const T*)v, cu_q, cu_kv, num_heads, \
                        num_kv_heads, head_size, q_stride, k_stride, v_stride, out_stride, sl2,          \
-                       sliding_window, num_sinks);                                                      \
+                       sliding_window, num_sinks, hpw);                                                 \
   } while (0)
   PE_DISPATCH_16(dtype, T, {
-    if (head_size <= 64) PE_LAUNCH_PW(T, 64, 2, 4, 2);
-    else if (head_size <= 128) PE_LAUNCH_PW(T, 128, 2, 4, 2);
-    else PE_LAUNCH_PW(T, 256, 1, 8, 2);
+    if (head_size <= 64) PE_LAUNCH_PW(T, 64, 1, 4, 2, 64);
+    else if (head_size > 128) PE_LAUNCH_PW(T, 256, 1, 8, 2, 64);
+    else if (wgs <= 256) PE_LAUNCH_PW(T, 128, 1, 4, 2, 64);
+    else if (span <= 288) PE_LAUNCH_PW(T, 128, 1, 4, 4, 32);
+    else PE_LAUNCH_PW(T, 128, 2, 4, 2, 64);
   });
 #undef PE_LAUNCH_PW
   return check_launch("prefill_window");
