@@ -160,6 +160,28 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_host = None
+
+
+def load_host():
+    """The host binding (csrc/host_binding.cpp): the operators that check their tensors in C++."""
+    global _host
+    if _host is None:
+        load()
+        path = os.path.join(_HERE, "_host.so")
+        if not os.path.exists(path):
+            raise PagedEvictLibraryError(f"{path} not found: the host binding is not built "
+                                         "(run `python -m vllm_paged_compression_amd.build`)")
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries have to be in the process first)
+        spec = importlib.util.spec_from_file_location("_host", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _host = mod
+    return _host
+
+
 def check(status: int, what: str = "") -> None:
     """Non-zero status -> RuntimeError (the counterpart of TORCH_CHECK in the reference ops)."""
     if status != 0:

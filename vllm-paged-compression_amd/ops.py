@@ -994,100 +994,8 @@ class DecodeLayerLauncher:
 
 
 # -------------------------------------------------------------------------------------- 8-bit cache, window
-_KV_FORMATS = {"fp8": _lib.PE_KV_FP8_E4M3, "fp8_e4m3": _lib.PE_KV_FP8_E4M3, "int8": _lib.PE_KV_INT8}
-_KV_STORAGE = {_lib.PE_KV_FP8_E4M3: (torch.float8_e4m3fn, torch.uint8), _lib.PE_KV_INT8: (torch.int8,)}
-
-
-def _launch(dev: torch.device, fn, what: str, *args) -> None:
-    """Call a C entry point on ``dev``'s current stream (the last argument) with ``dev`` current."""
-    if dev.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
-        return
-    with torch.cuda.device(dev):
-        _lib.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
-
-
-def _check_rows(what: str, name: str, t: torch.Tensor, heads: int, head_size: int) -> None:
-    """[rows, heads, head_size] whose rows are dense and 16-byte aligned."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_size:
-        raise RuntimeError(f"{what}: {name} must be [rows, {heads}, {head_size}]")
-    if t.numel() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_size)):
-        raise RuntimeError(f"{what}: the rows of {name} must be dense")
-    # (a tensor of one row is never stepped over: any row stride will do)
-    if t.numel() and (t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 8)):
-        raise RuntimeError(f"{what}: the rows of {name} must be 16-byte aligned")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
-
-
-def _check_paged(what: str, key_cache: torch.Tensor, value_cache: torch.Tensor, x: int,
-                 block_tables: torch.Tensor, seq_lens: torch.Tensor) -> Tuple[int, int, int, int]:
-    """(num_blocks, kv heads, head size, block size) of a paged cache and its tables."""
-    if key_cache.dim() != 5 or value_cache.dim() != 4:
-        raise RuntimeError(f"{what}: key_cache must be 5-d and value_cache 4-d")
-    nb, H, D, bs = value_cache.shape
-    if D % x or key_cache.shape != (nb, H, D // x, bs, x):
-        raise RuntimeError(f"{what}: key_cache must be [{nb}, {H}, {D}/{x}, {bs}, {x}]")
-    if key_cache.dtype != value_cache.dtype:
-        raise RuntimeError(f"{what}: key and value cache differ in dtype")
-    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
-        raise RuntimeError(f"{what}: caches must be contiguous")
-    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32:
-        raise RuntimeError(f"{what}: block_tables and seq_lens must be int32")
-    if block_tables.dim() != 2 or not block_tables.is_contiguous():
-        raise RuntimeError(f"{what}: block_tables must be contiguous [num_seqs, max_blocks]")
-    if seq_lens.dim() != 1 or seq_lens.shape[0] != block_tables.shape[0] or not seq_lens.is_contiguous():
-        raise RuntimeError(f"{what}: seq_lens must be contiguous [num_seqs]")
-    return nb, H, D, bs
-
-
-def _check_8bit(what: str, key_cache, value_cache, kv_scales, block_tables, seq_lens,
-                kv_cache_dtype: str, rows: torch.Tensor):
-    fmt = _KV_FORMATS.get(kv_cache_dtype)
-    if fmt is None:
-        raise ValueError(f"{what}: kv_cache_dtype must be one of {sorted(_KV_FORMATS)}, got {kv_cache_dtype!r}")
-    if key_cache.dtype not in _KV_STORAGE[fmt]:
-        raise RuntimeError(f"{what}: a {kv_cache_dtype} cache is held in "
-                           f"{' or '.join(map(str, _KV_STORAGE[fmt]))}, got {key_cache.dtype}")
-    if rows.dtype not in (torch.bfloat16, torch.float16):
-        raise RuntimeError(f"{what}: bfloat16 or float16 rows expected, got {rows.dtype}")
-    nb, H, D, bs = _check_paged(what, key_cache, value_cache, 16, block_tables, seq_lens)
-    if kv_scales.dtype != torch.float32 or kv_scales.shape != (nb, H, 2) or not kv_scales.is_contiguous():
-        raise RuntimeError(f"{what}: kv_scales must be contiguous float32 [{nb}, {H}, 2]")
-    return fmt, nb, H, D, bs
-
-
-def _check_new_rows(what: str, key, value, H: int, D: int) -> None:
-    _check_rows(what, "key", key, H, D)
-    _check_rows(what, "value", value, H, D)
-    if key.shape != value.shape or key.dtype != value.dtype:
-        raise RuntimeError(f"{what}: key and value differ in shape or dtype")
-
-
-def _check_decode(what: str, out, query, num_kv_heads: int, block_size: int, H: int, D: int, bs: int,
-                  seqs: int, sliding_window: int, num_sinks: int) -> None:
-    if num_kv_heads != H or block_size != bs:
-        raise RuntimeError(f"{what}: cache shape does not match num_kv_heads/block_size")
-    if query.dim() != 3 or query.shape[0] != seqs or query.shape[1] % H or query.shape[1] == 0:
-        raise RuntimeError(f"{what}: query must be [num_seqs, num_heads, head_size] with num_heads a "
-                           "multiple of num_kv_heads")
-    _check_rows(what, "query", query, query.shape[1], D)
-    if out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
-        raise RuntimeError(f"{what}: out must be contiguous, of query's shape and dtype")
-    if sliding_window < 0 or num_sinks < 0:
-        raise ValueError(f"{what}: sliding_window and num_sinks must not be negative")
-
-
-def _window_workspace(dev, S: int, Hq: int, Hkv: int, D: int, max_seq_len: int, window: int, sinks: int,
-                      fmt: int) -> Tuple[Optional[torch.Tensor], int]:
-    """Split-KV partials of one call: a buffer of its own from torch's allocator, so that calls on
-    two streams, or in two captured graphs, never share one."""
-    need = _lib.load().pe_paged_window_workspace_bytes(S, Hq, Hkv, D, max_seq_len, window, sinks, fmt)
-    return (torch.empty(need, dtype=torch.uint8, device=dev), need) if need > 0 else (None, 0)
-
-
+# These operators check their tensors in the host binding (csrc/host_binding.cpp): they are issued once
+# per layer, and checked here they would take longer than the smallest of them keep the GPU busy.
 def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
                            value_cache: torch.Tensor, kv_scales: torch.Tensor,
                            block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -1099,26 +1007,9 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, key_cache: to
     [nb, H_kv, 2].  Sequence s takes rows cu_q[s] .. cu_q[s+1]-1 (``cu_q=None``: row s) at the end of
     its seq_lens[s] tokens, which count them.  A block takes the smallest power of two that holds its
     tokens as scale; it begins anew when a call writes its offset 0, and its older codes are
-    re-expressed when a later row needs a larger scale."""
-    what = "reshape_and_cache_8bit"
-    fmt, nb, H, D, bs = _check_8bit(what, key_cache, value_cache, kv_scales, block_tables, seq_lens,
-                                    kv_cache_dtype, key)
-    _check_new_rows(what, key, value, H, D)
-    S, T = block_tables.shape[0], key.shape[0]
-    if cu_q is None:
-        if T != S:
-            raise RuntimeError(f"{what}: without cu_q key/value hold one row per sequence")
-    elif cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] != S + 1 or not cu_q.is_contiguous():
-        raise RuntimeError(f"{what}: cu_q must be contiguous int32 [num_seqs + 1]")
-    if max_q_len < 0:
-        raise ValueError(f"{what}: negative max_q_len")
-    dev = _need_gpu(key, value, key_cache, value_cache, kv_scales, block_tables, seq_lens, cu_q)
-    if S == 0 or T == 0:
-        return
-    _launch(dev, _lib.load().pe_reshape_and_cache_8bit, what, _p(key), _p(value), _p(key_cache),
-            _p(value_cache), _p(kv_scales), _p(block_tables), _p(seq_lens), _p(cu_q), S, T,
-            int(max_q_len), _row_stride(key), _row_stride(value), H, D, bs, nb, block_tables.shape[1],
-            H * D * bs, D * bs, _dtype_code(key), fmt)
+    re-expressed when a later row needs a larger scale.  Two sequences must not append to one block."""
+    (_lib._host or _lib.load_host()).reshape_and_cache_8bit(
+        key, value, key_cache, value_cache, kv_scales, block_tables, seq_lens, cu_q, max_q_len, kv_cache_dtype)
 
 
 def paged_attention_8bit(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor,
@@ -1129,20 +1020,9 @@ def paged_attention_8bit(out: torch.Tensor, query: torch.Tensor, key_cache: torc
     """Decode attention over an 8-bit paged cache: out[s] attends the seq_lens[s] tokens of table row
     s, or - with ``sliding_window`` > 0 - the last ``sliding_window`` of them and the first
     ``num_sinks``.  ``max_seq_len`` (an upper bound of seq_lens) sizes the split over the keys."""
-    what = "paged_attention_8bit"
-    fmt, nb, H, D, bs = _check_8bit(what, key_cache, value_cache, kv_scales, block_tables, seq_lens,
-                                    kv_cache_dtype, query)
-    S = block_tables.shape[0]
-    _check_decode(what, out, query, num_kv_heads, block_size, H, D, bs, S, sliding_window, num_sinks)
-    dev = _need_gpu(out, query, key_cache, value_cache, kv_scales, block_tables, seq_lens)
-    if S == 0:
-        return
-    Hq = query.shape[1]
-    ws, need = _window_workspace(dev, S, Hq, H, D, int(max_seq_len), sliding_window, num_sinks, fmt)
-    _launch(dev, _lib.load().pe_paged_decode_8bit, what, _p(out), _p(query), _p(key_cache),
-            _p(value_cache), _p(kv_scales), _p(block_tables), _p(seq_lens), S, Hq, H, D, bs, nb,
-            block_tables.shape[1], _row_stride(query), H * D * bs, D * bs, float(scale),
-            int(max_seq_len), sliding_window, num_sinks, _dtype_code(query), fmt, _p(ws), need)
+    (_lib._host or _lib.load_host()).paged_attention_8bit(
+        out, query, key_cache, value_cache, kv_scales, num_kv_heads, scale, block_tables, seq_lens, block_size,
+        max_seq_len, kv_cache_dtype, sliding_window, num_sinks)
 
 
 def decode_step_8bit(out: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -1152,24 +1032,9 @@ def decode_step_8bit(out: torch.Tensor, query: torch.Tensor, key: torch.Tensor, 
                      sliding_window: int = 0, num_sinks: int = 0) -> None:
     """One decode layer over an 8-bit paged cache: ``reshape_and_cache_8bit`` of one row per sequence
     (key/value [S, H_kv, D], seq_lens counting it), then ``paged_attention_8bit``."""
-    what = "decode_step_8bit"
-    fmt, nb, H, D, bs = _check_8bit(what, key_cache, value_cache, kv_scales, block_tables, seq_lens,
-                                    kv_cache_dtype, query)
-    S = block_tables.shape[0]
-    _check_decode(what, out, query, num_kv_heads, block_size, H, D, bs, S, sliding_window, num_sinks)
-    _check_new_rows(what, key, value, H, D)
-    if key.shape[0] != S or key.dtype != query.dtype:
-        raise RuntimeError(f"{what}: key/value must be [num_seqs, num_kv_heads, head_size] of query's dtype")
-    dev = _need_gpu(out, query, key, value, key_cache, value_cache, kv_scales, block_tables, seq_lens)
-    if S == 0:
-        return
-    Hq = query.shape[1]
-    ws, need = _window_workspace(dev, S, Hq, H, D, int(max_seq_len), sliding_window, num_sinks, fmt)
-    _launch(dev, _lib.load().pe_decode_step_8bit, what, _p(out), _p(query), _p(key), _p(value),
-            _p(key_cache), _p(value_cache), _p(kv_scales), _p(block_tables), _p(seq_lens), S, Hq, H, D,
-            bs, nb, block_tables.shape[1], _row_stride(query), _row_stride(key), _row_stride(value),
-            H * D * bs, D * bs, float(scale), int(max_seq_len), sliding_window, num_sinks,
-            _dtype_code(query), fmt, _p(ws), need)
+    (_lib._host or _lib.load_host()).decode_step_8bit(
+        out, query, key, value, key_cache, value_cache, kv_scales, num_kv_heads, scale, block_tables, seq_lens,
+        block_size, max_seq_len, kv_cache_dtype, sliding_window, num_sinks)
 
 
 def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor,
@@ -1179,21 +1044,9 @@ def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: to
     """Decode attention over a 16-bit paged cache through a window: out[s] attends the last
     ``sliding_window`` of its seq_lens[s] tokens and the first ``num_sinks`` (0: every token).
     Blocks without such a token are not read and their table entries may be stale."""
-    what = "paged_attention_window"
-    if query.dtype not in (torch.bfloat16, torch.float16) or key_cache.dtype != query.dtype:
-        raise RuntimeError(f"{what}: query and caches must share bfloat16 or float16")
-    nb, H, D, bs = _check_paged(what, key_cache, value_cache, 8, block_tables, seq_lens)
-    S = block_tables.shape[0]
-    _check_decode(what, out, query, num_kv_heads, block_size, H, D, bs, S, sliding_window, num_sinks)
-    dev = _need_gpu(out, query, key_cache, value_cache, block_tables, seq_lens)
-    if S == 0:
-        return
-    Hq = query.shape[1]
-    ws, need = _window_workspace(dev, S, Hq, H, D, int(max_seq_len), sliding_window, num_sinks, _lib.PE_KV_SAME)
-    _launch(dev, _lib.load().pe_paged_decode_window, what, _p(out), _p(query), _p(key_cache),
-            _p(value_cache), _p(block_tables), _p(seq_lens), S, Hq, H, D, bs, nb, block_tables.shape[1],
-            _row_stride(query), H * D * bs, D * bs, float(scale), int(max_seq_len), sliding_window,
-            num_sinks, _dtype_code(query), _p(ws), need)
+    (_lib._host or _lib.load_host()).paged_attention_window(
+        out, query, key_cache, value_cache, num_kv_heads, scale, block_tables, seq_lens, block_size, max_seq_len,
+        sliding_window, num_sinks)
 
 
 def prefill_window(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_q: torch.Tensor,
@@ -1203,36 +1056,8 @@ def prefill_window(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     min(i, Lkv-1) with j > i - ``sliding_window`` (0: all of them) or j < ``num_sinks``; a query that
     sees none gets zeros.  query [Tq, Hq, D], key/value [Tkv, Hkv, D] bf16 or f16; cu_q/cu_kv int32
     prefix sums; ``max_q_len`` = the longest request."""
-    what = "prefill_window"
-    if query.dim() != 3 or key.dim() != 3 or key.shape[1] == 0 or query.shape[1] % key.shape[1] \
-            or value.shape != key.shape:
-        raise RuntimeError(f"{what}: query [Tq, Hq, D], key/value [Tkv, Hkv, D] expected, Hq a multiple of Hkv")
-    (Tq, Hq, D), Hkv = query.shape, key.shape[1]
-    if query.dtype not in (torch.bfloat16, torch.float16) or key.dtype != query.dtype or value.dtype != query.dtype:
-        raise RuntimeError(f"{what}: query, key and value must share bfloat16 or float16")
-    for name, t, heads in (("query", query, Hq), ("key", key, Hkv), ("value", value, Hkv)):
-        _check_rows(what, name, t, heads, D)
-    for t in (cu_q, cu_kv):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < 1 or t.shape != cu_q.shape or not t.is_contiguous():
-            raise RuntimeError(f"{what}: cu_q/cu_kv must be contiguous int32 [num_requests + 1]")
-    if sliding_window < 0 or num_sinks < 0 or max_q_len < 0:
-        raise ValueError(f"{what}: max_q_len, sliding_window and num_sinks must not be negative")
-    if out is not None:
-        _check_rows(what, "out", out, Hq, D)
-        if out.shape != query.shape or out.dtype != query.dtype:
-            raise RuntimeError(f"{what}: out must have query's shape and dtype")
-    dev = _need_gpu(query, key, value, cu_q, cu_kv, out)
-    if out is None:
-        out = torch.empty((Tq, Hq, D), dtype=query.dtype, device=dev)
-    if Tq == 0 or cu_q.shape[0] == 1:
-        return out
-    if key.shape[0] == 0:   # nothing to attend
-        return out.zero_()
-    _launch(dev, _lib.load().pe_prefill_window, what, _p(out), _p(query), _p(key), _p(value), _p(cu_q),
-            _p(cu_kv), cu_q.shape[0] - 1, int(max_q_len), Hq, Hkv, D, _row_stride(query),
-            _row_stride(key), _row_stride(value), _row_stride(out), float(scale), sliding_window,
-            num_sinks, _dtype_code(query))
-    return out
+    return (_lib._host or _lib.load_host()).prefill_window(
+        query, key, value, cu_q, cu_kv, max_q_len, scale, sliding_window, num_sinks, out)
 
 
 # -------------------------------------------------------------------------------------- torch.library
