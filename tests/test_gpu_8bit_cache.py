@@ -258,14 +258,43 @@ def test_attention_long_sequences_few_and_many(ops, window, sinks):
     g = torch.Generator().manual_seed(11)
     H, D, bs = 1, 128, 16
     kc, vc, sc, t = filled(g, [5003], H, D, bs, "fp8")
-    for seqs in (1, 3, 300):
+    for seqs in (1, 3, 20, 300):
         ln = torch.full((seqs,), 5003, dtype=torch.int32)
         q = rows(g, 3, 4, D, torch.bfloat16)[torch.arange(seqs) % 3].contiguous()
         out, _ = run_attention(ops, q, kc, vc, sc, t.expand(seqs, -1).contiguous(), ln, "fp8", window, sinks)
-        ref, bound = plain.decode(q[:3], kc, vc, sc, t.expand(3, -1)[:seqs], ln[:3], window, sinks, D ** -0.5)
-        plain.assert_within(out[:3], ref[:seqs], bound[:seqs], f"{seqs} sequences")
-        if seqs == 300:
-            assert torch.equal(out[3:], out[:3][torch.arange(3, 300) % 3]), "a row's result hangs on its place"
+        n = min(seqs, 3)
+        ref, bound = plain.decode(q[:n], kc, vc, sc, t.expand(n, -1), ln[:n], window, sinks, D ** -0.5)
+        plain.assert_within(out[:n], ref, bound, f"{seqs} sequences")
+        if seqs > 3:
+            assert torch.equal(out[3:], out[:3][torch.arange(3, seqs) % 3]), "a row's result hangs on its place"
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_attention_and_step_many_short_sequences(ops, fmt):
+    """Launches of 100 workgroups with some tiles each (the wide workgroups), attention and step."""
+    g = torch.Generator().manual_seed(13)
+    H, D, bs, S = 1, 64, 16, 100
+    lens = [850 + 5 * i % 61 for i in range(S)]
+    kc, vc, sc, t = filled(g, [912] * 3, H, D, bs, fmt, spare=S + 5)
+    full = t[torch.arange(S) % 3].clone()
+    # the sequences share their full blocks; each has a last block of its own
+    free = torch.tensor([b for b in range(vc.shape[0]) if b not in set(t.flatten().tolist())], dtype=torch.int32)
+    for s, n in enumerate(lens):
+        own, old = int(free[s]), int(full[s, n // bs])
+        kc[own], vc[own], sc[own] = kc[old], vc[old], sc[old]
+        full[s, n // bs] = own
+    ln = torch.tensor(lens, dtype=torch.int32)
+    q = rows(g, S, 4, D, torch.bfloat16)
+    out, _ = run_attention(ops, q, kc, vc, sc, full, ln, fmt, 0, 0)
+    ref, bound = plain.decode(q[:8], kc, vc, sc, full, ln[:8], 0, 0, D ** -0.5)
+    plain.assert_within(out[:8], ref, bound, "attention")
+    k, v = rows(g, S, H, D, torch.bfloat16, 3.0), rows(g, S, H, D, torch.bfloat16, 3.0)
+    ln = ln + 1
+    out, dev = run_attention(ops, q, kc, vc, sc, full, ln, fmt, 0, 0, step=(k, v))
+    plain.write(k, v, kc, vc, sc, full, ln, None, fmt)
+    assert all(same_bits(a, b) for a, b in zip(dev, (kc, vc, sc)))
+    ref, bound = plain.decode(q[:8], kc, vc, sc, full, ln[:8], 0, 0, D ** -0.5)
+    plain.assert_within(out[:8], ref, bound, "step")
 
 
 def test_attention_reports_bad_blocks_and_lengths(ops):

@@ -105,18 +105,13 @@ __global__ __launch_bounds__(W8_THREADS) void cache8_write_kernel(
       const float f = ks_old * ki;
       for (int it = tid; it < (head_size >> 4) * o0 * 4; it += W8_THREADS) {
         const int c = it / (o0 * 4), w = it % (o0 * 4);
-        uint32_t* p = reinterpret_cast<uint32_t*>(kb + (int64_t)c * block_size * 16) + w;
-        const uint32_t q = *p;
-        *p = encode4<F>(code_value<F>(q & 255u) * f, code_value<F>((q >> 8) & 255u) * f,
-                        code_value<F>((q >> 16) & 255u) * f, code_value<F>(q >> 24) * f);
+        reencode_word<F>(reinterpret_cast<uint32_t*>(kb + c * block_size * 16) + w, f);
       }
     }
     if (vs_old > 0.f && vs > vs_old) {
       const float f = vs_old * vi;
-      for (int it = tid; it < head_size * o0; it += W8_THREADS) {
-        uint8_t* p = vb + (it / o0) * block_size + it % o0;
-        *p = (uint8_t)encode4<F>(code_value<F>(*p) * f, 0.f, 0.f, 0.f);
-      }
+      for (int it = tid; it < head_size * o0; it += W8_THREADS)
+        reencode_byte<F>(vb + (it / o0) * block_size + it % o0, f);
     }
     if (tid == 0) {
       sc[0] = ks;

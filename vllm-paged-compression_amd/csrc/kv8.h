@@ -77,6 +77,18 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
   }
 }
 
+// older codes of a block whose scale grew, f = old scale / new scale
+template <typename F>
+__device__ __forceinline__ void reencode_word(uint32_t* p, float f) {
+  const uint32_t q = *p;
+  *p = encode4<F>(code_value<F>(q & 255u) * f, code_value<F>((q >> 8) & 255u) * f,
+                  code_value<F>((q >> 16) & 255u) * f, code_value<F>(q >> 24) * f);
+}
+template <typename F>
+__device__ __forceinline__ void reencode_byte(uint8_t* p, float f) {
+  *p = (uint8_t)encode4<F>(code_value<F>(*p) * f, 0.f, 0.f, 0.f);
+}
+
 // smallest power of two s with amax / s <= F::MAX, at least 2^-100 (its reciprocal and the
 // quotients stay far from f32's ends); 0 for amax = 0.  amax is finite and not negative.
 template <typename F>

@@ -1,30 +1,70 @@
 // Entry points of the windowed and the 8-bit decode attention (kernel: paged_window_kernel.h)
 //   pe_paged_decode_window   16-bit cache, sliding window + sink tokens
 //   pe_paged_decode_8bit     8-bit cache, with or without a window
-//   pe_decode_step_8bit      KV write of the step's token + the attention
+//   pe_decode_step_8bit      KV write of the step's token + the attention, in one launch for head sizes up to
+//                            128 with up to 16 query heads per KV head
+#include <initializer_list>
+
 #include "paged_window_kernel.h"
 
 namespace pe {
 
-int launch_window_16(const WinArgs& a, int head_size, int block_size, int dtype, dim3 grid, hipStream_t st);
-int launch_window_fp8(const WinArgs& a, int head_size, int block_size, int dtype, dim3 grid, hipStream_t st);
-int launch_window_int8(const WinArgs& a, int head_size, int block_size, int dtype, dim3 grid, hipStream_t st);
+int launch_window_16(const WinArgs& a, int head_size, int block_size, int waves, int dtype, dim3 grid, hipStream_t st);
+int launch_window_fp8(const WinArgs& a, int head_size, int block_size, int waves, int dtype, dim3 grid, hipStream_t st);
+int launch_window_int8(const WinArgs& a, int head_size, int block_size, int waves, int dtype, dim3 grid, hipStream_t st);
+int launch_step_fp8(const WinArgs& a, int head_size, int block_size, int waves, int dtype, dim3 grid, hipStream_t st);
+int launch_step_int8(const WinArgs& a, int head_size, int block_size, int waves, int dtype, dim3 grid, hipStream_t st);
 int window_16_diag_fetch(unsigned int* out, int reset);
 int window_fp8_diag_fetch(unsigned int* out, int reset);
 int window_int8_diag_fetch(unsigned int* out, int reset);
+int step_fp8_diag_fetch(unsigned int* out, int reset);
+int step_int8_diag_fetch(unsigned int* out, int reset);
 
 int window_diag_fetch(unsigned int* out, int reset) {
-  unsigned int a = 0, b = 0, c = 0;
-  if (int rc = window_16_diag_fetch(&a, reset)) return rc;
-  if (int rc = window_fp8_diag_fetch(&b, reset)) return rc;
-  if (int rc = window_int8_diag_fetch(&c, reset)) return rc;
-  *out = a | b | c;
+  *out = 0;
+  for (auto fetch : {window_16_diag_fetch, window_fp8_diag_fetch, window_int8_diag_fetch, step_fp8_diag_fetch,
+                     step_int8_diag_fetch}) {
+    unsigned int one = 0;
+    if (int rc = fetch(&one, reset)) return rc;
+    *out |= one;
+  }
   return PE_OK;
 }
 
-static int window_splits(int num_seqs, int num_heads, int num_kv_heads, int max_seq_len, int window,
-                         int sinks, int kv_format) {
-  return 1;
+// Workgroup width (waves) and number of splits over the keys of a launch.  A split costs a merge launch
+// (about 2.5 us); a wave takes its tiles (16 KiB at head size 128) one memory round trip after the
+// other, so a launch that cannot fill the chip wants one tile per wave.  Measured on MI355X
+// (graph-replayed, us; waves/splits; workgroups without splits x tiles of a sequence):
+//   512 x 112 (64 x 8192 tokens, 8 bit): 4/1 154, 4/2 156, 8/1 172; 512 x 32: 42 / 45 / 49; 512 x 13: 19 / 24 / 22
+//   512 x 33 (16 bit): 4/1 45, 4/2 49, 8/1 52; 512 x 64: 75 / 80 / 86; 2048 x 4: 22 / 41 / 43
+//   256 x 13: 4/1 12.5, 8/1 13.1, 4/2 15.0; 192 x 65 (head 64): 4/1 29, 4/2 22, 4/4 21, 8/1 21
+//   128 x 128: 4/1 58, 4/2 43, 4/4 43, 8/1 55; 32 x 512: 4/4 60, 4/8 43, 8/8 50
+//    64 x 65: 4/4 16.7, 4/6 17.6, 4/8 15.7, 8/1 22; 64 x 49: 4/4 14.5, 4/6 15.2, 4/8 15.9, 8/1 19; 64 x 25: 4/4 9.4, 8/1 9.4
+//     8 x 65: 4/8 11.1, 8/8 8.9, 8/9 8.2; 8 x 25: 4/4 8.3, 4/7 6.8, 8/1 8.0; 12 x 13: 4/1 8.2, 4/4 6.7, 8/1 7.5
+struct WinShape {
+  int waves, splits;
+};
+static WinShape window_shape(int num_seqs, int num_heads, int num_kv_heads, int max_seq_len, int window,
+                             int sinks, int kv_format) {
+  const int gqa = num_heads / num_kv_heads;
+  const int64_t wgs = (int64_t)num_seqs * num_kv_heads * ((gqa + 15) / 16);
+  const int tok = kv_format == PE_KV_SAME ? 32 : 64;
+  const int64_t seen = window > 0 && (int64_t)window + sinks < max_seq_len ? (int64_t)window + sinks : max_seq_len;
+  // (a window and its sinks may each begin and end inside a tile)
+  const int64_t tiles = (seen + tok - 1) / tok + (window > 0 && seen < max_seq_len ? 1 + (sinks > 0) : 0);
+  WinShape s{4, 1};
+  if (tiles <= 4) return s;
+  if (wgs >= 256) return s;  // the chip is full
+  if (wgs * tiles <= 1024) {  // one tile per wave
+    if (tiles > 32) s.waves = 8;
+    s.splits = (int)((tiles + s.waves - 1) / s.waves);
+  } else if (wgs * tiles <= 4352 && tiles <= 32) {
+    s.waves = 8;
+  } else {  // bound by bandwidth: a workgroup per CU
+    s.splits = (int)((256 + wgs - 1) / wgs);
+  }
+  if (s.splits > WIN_MAX_SPLITS) s.splits = WIN_MAX_SPLITS;
+  return s;
 }
 
 static int check_window(const char* who, int window, int sinks) {
@@ -39,7 +79,9 @@ static int window_decode(const char* who, void* out, const void* query, const vo
                          int head_size, int block_size, int64_t num_blocks, int table_width,
                          int64_t q_stride, int64_t kv_block_stride, int64_t kv_head_stride, float scale,
                          int max_seq_len, int window, int sinks, int dtype, int kv_format,
-                         void* workspace, int64_t workspace_bytes, void* stream) {
+                         void* workspace, int64_t workspace_bytes, void* stream,
+                         const void* new_key = nullptr, const void* new_value = nullptr,
+                         int64_t new_k_stride = 0, int64_t new_v_stride = 0) {
   PE_REQUIRE(out && query && key_cache && value_cache && block_tables && seq_lens, PE_ERR_INVALID_ARG,
              "%s: null pointer", who);
   PE_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0, PE_ERR_INVALID_ARG,
@@ -50,7 +92,8 @@ static int window_decode(const char* who, void* out, const void* query, const vo
   const int gqa = num_heads / num_kv_heads, groups = (gqa + 15) / 16;
   PE_REQUIRE(num_seqs <= 65535 && (int64_t)num_kv_heads * groups <= 65535, PE_ERR_UNSUPPORTED,
              "%s: grid too large", who);
-  const int splits = window_splits(num_seqs, num_heads, num_kv_heads, max_seq_len, window, sinks, kv_format);
+  const WinShape shape = window_shape(num_seqs, num_heads, num_kv_heads, max_seq_len, window, sinks, kv_format);
+  const int splits = shape.splits, waves = shape.waves;
   if (splits > 1) {
     const int64_t need = (int64_t)splits * num_seqs * num_heads * win_ws_stride(head_size) * 4;
     PE_REQUIRE(workspace && workspace_bytes >= need, PE_ERR_WORKSPACE, "%s needs %lld workspace bytes, got %lld",
@@ -58,13 +101,28 @@ static int window_decode(const char* who, void* out, const void* query, const vo
   }
   const WinArgs a{out, (float*)workspace, query, key_cache, value_cache, kv_scales, block_tables, seq_lens,
                   num_heads, num_kv_heads, table_width, window, sinks, splits, groups, num_blocks, q_stride,
-                  kv_block_stride, kv_head_stride, scale * 1.4426950408889634f};
+                  kv_block_stride, kv_head_stride, scale * 1.4426950408889634f,
+                  new_key, new_value, new_k_stride, new_v_stride};
   const dim3 grid((unsigned)splits, (unsigned)(num_kv_heads * groups), (unsigned)num_seqs);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  // The row is written by a launch of its own where several workgroups read the block that it joins (more
+  // than 16 query heads on a KV head) and where the kernel has no registers left for it
+  const bool step = new_key != nullptr && groups == 1 && head_size <= 128;
+  if (new_key != nullptr && !step) {
+    if (int rc = pe_reshape_and_cache_8bit(new_key, new_value, const_cast<void*>(key_cache),
+                                           const_cast<void*>(value_cache), const_cast<float*>(kv_scales), block_tables,
+                                           seq_lens, nullptr, num_seqs, num_seqs, 1, new_k_stride, new_v_stride,
+                                           num_kv_heads, head_size, block_size, num_blocks, table_width,
+                                           kv_block_stride, kv_head_stride, dtype, kv_format, stream))
+      return rc;
+  }
   int rc;
-  if (kv_format == PE_KV_FP8_E4M3) rc = launch_window_fp8(a, head_size, block_size, dtype, grid, st);
-  else if (kv_format == PE_KV_INT8) rc = launch_window_int8(a, head_size, block_size, dtype, grid, st);
-  else rc = launch_window_16(a, head_size, block_size, dtype, grid, st);
+  if (kv_format == PE_KV_FP8_E4M3)
+    rc = (step ? launch_step_fp8 : launch_window_fp8)(a, head_size, block_size, waves, dtype, grid, st);
+  else if (kv_format == PE_KV_INT8)
+    rc = (step ? launch_step_int8 : launch_window_int8)(a, head_size, block_size, waves, dtype, grid, st);
+  else
+    rc = launch_window_16(a, head_size, block_size, waves, dtype, grid, st);
   if (rc) return rc;
   return check_launch(who);
 }
@@ -77,7 +135,8 @@ int64_t pe_paged_window_workspace_bytes(int num_seqs, int num_heads, int num_kv_
                                         int max_seq_len, int sliding_window, int num_sinks, int kv_format) {
   using namespace pe;
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0) return 0;
-  const int splits = window_splits(num_seqs, num_heads, num_kv_heads, max_seq_len, sliding_window, num_sinks, kv_format);
+  const int splits =
+      window_shape(num_seqs, num_heads, num_kv_heads, max_seq_len, sliding_window, num_sinks, kv_format).splits;
   return splits <= 1 ? 0 : (int64_t)splits * num_seqs * num_heads * win_ws_stride(head_size) * 4;
 }
 
@@ -136,17 +195,22 @@ int pe_decode_step_8bit(void* out, const void* query, const void* new_key, const
                         int64_t kv_block_stride, int64_t kv_head_stride, float scale, int max_seq_len,
                         int sliding_window, int num_sinks, int dtype, int kv_format, void* workspace,
                         int64_t workspace_bytes, void* stream) {
-  if (int rc = pe_reshape_and_cache_8bit(new_key, new_value, key_cache, value_cache, kv_scales, block_tables,
-                                         seq_lens, nullptr, num_seqs, num_seqs, 1, new_k_stride, new_v_stride,
-                                         num_kv_heads, head_size, block_size, num_blocks,
-                                         max_num_blocks_per_seq, kv_block_stride, kv_head_stride, dtype,
-                                         kv_format, stream))
+  using namespace pe;
+  const char* who = "decode_step_8bit";
+  PE_REQUIRE(num_seqs >= 0, PE_ERR_INVALID_ARG, "%s: negative num_seqs", who);
+  if (num_seqs == 0) return PE_OK;
+  PE_REQUIRE(kv_scales && new_key && new_value, PE_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (int rc = check_window(who, sliding_window, num_sinks)) return rc;
+  if (int rc = check_cache8(who, key_cache, value_cache, kv_scales, num_kv_heads, head_size, block_size,
+                            num_blocks, max_num_blocks_per_seq, kv_block_stride, kv_head_stride, dtype, kv_format))
     return rc;
-  return pe_paged_decode_8bit(out, query, key_cache, value_cache, kv_scales, block_tables, seq_lens, num_seqs,
-                              num_heads, num_kv_heads, head_size, block_size, num_blocks,
-                              max_num_blocks_per_seq, q_stride, kv_block_stride, kv_head_stride, scale,
-                              max_seq_len, sliding_window, num_sinks, dtype, kv_format, workspace,
-                              workspace_bytes, stream);
+  PE_REQUIRE(new_k_stride % 8 == 0 && new_v_stride % 8 == 0 && ((uintptr_t)new_key | (uintptr_t)new_value) % 16 == 0,
+             PE_ERR_INVALID_ARG, "%s: key/value rows must be 16-byte aligned", who);
+  return window_decode(who, out, query, key_cache, value_cache, kv_scales, block_tables, seq_lens, num_seqs,
+                       num_heads, num_kv_heads, head_size, block_size, num_blocks, max_num_blocks_per_seq,
+                       q_stride, kv_block_stride, kv_head_stride, scale, max_seq_len, sliding_window,
+                       num_sinks, dtype, kv_format, workspace, workspace_bytes, stream, new_key, new_value,
+                       new_k_stride, new_v_stride);
 }
 
 }  // extern "C"

@@ -5,22 +5,27 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q.k_j - max),  j in the visible set:
 //   j < len and (window == 0 or j >= len - window or j < sinks);  nothing visible: o = 0.
 //
-// Layout.  A tile is four units of U = 16 / (element bytes) tokens (8 in 16 bits, 16 in 8 bits).
-// The 16x16x32 matrix instruction computes S^T = K.Q^T with the tile's tokens as rows: row 4g + r
-// of row block b is token 4b + r of unit g, so lane group g (16 lanes, one per query head) ends up
-// with the scores of unit g's tokens, in order.  That is the order in which one 16-byte piece of a
-// value row holds them, so P meets V in O^T += V^T.P^T without moving across lanes, every load is
-// 16 bytes per lane, and with 8-bit elements a lane's tokens share one block's scales.
-//   K: lane (g, c) loads chunk 4*kk + g of token 4b + (c & 3) of unit c >> 2 (64-byte runs)
-//   V: lane (g, c) loads row 16*dt + c of unit g
+// Layout.  A tile is NG groups of 16 tokens.  The 16x16x32 matrix instruction computes S^T = K.Q^T
+// with a group's tokens as rows: lane (g, c) (c = query head) ends up with the scores of tokens
+// 4g .. 4g+3 of every group.  A group lies in one block (in two with 8-token blocks), so block ids and
+// 8-bit scales are wave-uniform.
+//   K: lane (g, c) loads the 16-byte chunk 4*kk + g of token c: 1 KiB in one piece with 16-token blocks
+//   V, 16 bits: lane (g, c) loads tokens 4g .. 4g+3 (8 bytes) of row 16*dt + c of a group.  Two groups
+//     make one k-step of O^T += V^T.P^T whose slots are ordered so that P is used where it lies.
+//   V, 8 bits: lane (g, c) loads all 16 tokens (16 bytes) of row 16*dt + c of group g, and P goes to
+//     the lane group of its tokens by a 4x4 transpose of row swaps (8 per tile of 64 tokens).  With P
+//     left where it lies the loads are 4 bytes: 260 instead of 168 us on 945 MB.
 // 8-bit codes are converted to the query's type exactly; K's scale multiplies the f32 scores, V's
 // scale the probabilities.
 #pragma once
+#include <type_traits>
+
 #include "kv8.h"
 
 namespace pe {
 
 constexpr float WIN_NEG = -1.0e30f;
+constexpr int WIN_MAX_SPLITS = 32;
 
 // Conditions a launch survives (this translation unit's copy; read through pe_device_diagnostics)
 static __device__ unsigned int window_diag_word;
@@ -34,9 +39,18 @@ struct WinArgs {
   int num_heads, num_kv_heads, table_width, window, sinks, num_splits, head_groups;
   int64_t num_blocks, q_stride, kv_block_stride, kv_head_stride;  // strides in elements
   float scale_log2;
+  // pe_decode_step_8bit only
+  const void *new_key, *new_value;
+  int64_t new_k_stride, new_v_stride;
 };
 
 __host__ __device__ inline int64_t win_ws_stride(int head_size) { return head_size + 2; }
+
+template <bool NT, typename V>
+__device__ __forceinline__ V win_load(const V* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
 
 // max over the four lanes l, l^16, l^32, l^48 by row swaps (no LDS round trip)
 __device__ __forceinline__ float win_max_groups(float x) {
@@ -47,6 +61,8 @@ __device__ __forceinline__ float win_max_groups(float x) {
   auto b = __builtin_amdgcn_permlane16_swap(u, u, false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
 
 // The tiles of a sequence that hold visible tokens: [0, sink_tiles) and [first, first + window
 // tiles); tokens are visible when tok < len and (tok >= lo or tok < sink_end).
@@ -67,26 +83,34 @@ __host__ __device__ inline WinRange win_range(int len, int window, int sinks) {
   return r;
 }
 
-// T: query / output type; C: cache element (T, Fp8 or Int8); D: head size; BLK: tokens per block
-template <typename T, typename C, int D, int WAVES, int BLK>
+// T: query / output type; C: cache element (T, Fp8 or Int8); D: head size; BLK: tokens per block.
+// STEP (pe_decode_step_8bit): the sequence's last token is appended first, as pe_reshape_and_cache_8bit
+// does it.  Its block lies in the last tile, which one wave owns: that wave encodes the row, puts it
+// (and, where the block's scale grows, the re-expressed older codes) into the tile's registers and into
+// the cache, and goes on with the attention.  No other wave of the launch touches the block.
+template <typename T, typename C, int D, int WAVES, int BLK, bool STEP>
 __global__ __launch_bounds__(WAVES * 64, 2) void paged_window_kernel(const WinArgs a) {
   using TR = Traits<T>;
   using vec8 = typename TR::vec8;
   constexpr bool Q8 = !__is_same(C, T);
-  constexpr int ES = Q8 ? 1 : 2;          // bytes per cache element
-  constexpr int U = 16 / ES;              // tokens per unit
-  constexpr int TOK = 4 * U;              // tokens per tile
-  constexpr int NB = U / 4;               // row blocks of S^T
-  constexpr int NP = U / 8;               // P.V k-steps
-  constexpr int KC = (D * ES + 63) / 64;  // K chunks per lane and token
+  constexpr int ES = Q8 ? 1 : 2;              // bytes per cache element
+  constexpr int NG = Q8 ? 4 : 2;              // 16-token groups per tile
+  constexpr int TOK = 16 * NG;                // tokens per tile
+  constexpr int EPC = 16 / ES;                // elements per 16-byte chunk
+  constexpr int CHUNKS = D / EPC;             // chunks of a K row
+  constexpr int KC = (CHUNKS + 3) / 4;        // chunks per lane and token
   constexpr int DT = (D + 15) / 16;
-  constexpr int CHUNKS = D * ES / 16;     // chunks of a K row
-  constexpr int PB = BLK < U ? 2 : 1;     // blocks per unit
-  static_assert(D * ES % 16 == 0 && BLK * PB >= U, "head size / block size");
+  constexpr int PB = BLK == 8 ? 2 : 1;        // blocks per group
+  // K/V loads of the throughput shape carry the non-temporal hint (945 MB: 168 against 187 us); the
+  // latency shape serves launches of a few megabytes, which run faster with plain loads
+  constexpr bool STREAM = WAVES < 8;
+  static_assert(D % EPC == 0 && (BLK == 8 || BLK == 16 || BLK == 32), "head size / block size");
+  constexpr int NV = Q8 ? 1 : NG;             // pieces of a value row per lane and tile
+  using VP = typename std::conditional<Q8, u32x4, u32x2>::type;
 
   const int split = blockIdx.x;
   const int kvh = blockIdx.y / a.head_groups, hgrp = blockIdx.y % a.head_groups;
-  const int seq = blockIdx.z;
+  const int seq = blockIdx.z, num_seqs = gridDim.z;
   const int gqa = a.num_heads / a.num_kv_heads;
   const int head0 = kvh * gqa + hgrp * 16;
   const int nh = min(16, gqa - hgrp * 16);  // query heads of this workgroup
@@ -94,104 +118,144 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_window_kernel(const WinAr
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
 
-  const int32_t* table = a.block_tables + (int64_t)seq * a.table_width;
-  const int raw_len = a.seq_lens[seq];
+  // Ids of the blocks of a tile's groups, requested a tile ahead through the scalar cache: they are
+  // wave-uniform, and a vector load would queue behind (and so wait for) the tiles in flight.  The
+  // first ones do not wait for the sequence's length unless there is a window.
+  typedef const __attribute__((address_space(4))) int32_t* ConstInt;
+  const ConstInt table = (ConstInt)(a.block_tables + (int64_t)seq * a.table_width);
+  struct Ids {
+    int e[NG * PB];
+  };
+  auto load_ids = [&](int tile) {
+    Ids id;
+#pragma unroll
+    for (int e = 0; e < NG * PB; ++e)
+      id.e[e] = table[min((tile * NG * PB + e) * (16 / PB) / BLK, a.table_width - 1)];
+    return id;
+  };
+  // the waves of all splits take the tiles in turn
+  const int i0 = split * WAVES + wave, step = WAVES * a.num_splits;
+  Ids ids = load_ids(a.window == 0 ? i0 : 0);
+  const int raw_len = ((ConstInt)a.seq_lens)[seq];
   const int64_t most = (int64_t)a.table_width * BLK;
   const int len = raw_len > most ? (int)most : max(raw_len, 0);
-  if (raw_len > most && threadIdx.x == 0 && split == 0 && blockIdx.y == 0)
-    atomicOr(&window_diag_word, (unsigned)PE_DIAG_DECODE_LEN_CLAMPED);
+  uint32_t diag = raw_len > most ? PE_DIAG_DECODE_LEN_CLAMPED : 0;
   const WinRange R = win_range<TOK>(len, a.window, a.sinks);
-  const int per_split = (R.tiles + a.num_splits - 1) / a.num_splits;
-  const int i_begin = split * per_split, i_end = min(R.tiles, i_begin + per_split);
+  // STEP: the last tile, which takes the new row, is the first one of the last wave (the one with the
+  // fewest tiles); it changes places with the tile that is there in order
+  const int early = STEP ? min(step, R.tiles) - 1 : 0;
+  auto at = [&](int i) { return R.tile(!STEP ? i : i == early ? R.tiles - 1 : i == R.tiles - 1 ? early : i); };
+  if (i0 < R.tiles && (a.window != 0 || at(i0) != i0)) ids = load_ids(at(i0));
+  auto visible = [&](int tok) { return (int)(tok < R.len) & ((int)(tok >= R.lo) | (int)(tok < R.sink_end)); };
 
   // ---- Q: the lane's chunks of head c, matched to the K chunks -------------------------------
-  vec8 qf[KC][ES == 1 ? 2 : 1];
+  vec8 qf[KC][Q8 ? 2 : 1];
   {
-    const T* qp = (const T*)a.query + (int64_t)seq * a.q_stride + (int64_t)(head0 + c) * D;
+    // (a lane without a head or a chunk reads a valid one and drops it)
+    const T* qp = (const T*)a.query + (int64_t)seq * a.q_stride + (int64_t)(head0 + min(c, nh - 1)) * D;
 #pragma unroll
     for (int kk = 0; kk < KC; ++kk)
 #pragma unroll
       for (int e = 0; e < (Q8 ? 2 : 1); ++e) {
-        u32x4 raw = {0u, 0u, 0u, 0u};
-        if (c < nh && 4 * kk + g < CHUNKS)
-          raw = *reinterpret_cast<const u32x4*>(qp + (4 * kk + g) * U + 8 * e);
-        qf[kk][e] = __builtin_bit_cast(vec8, raw);
+        const bool in = c < nh && 4 * kk + g < CHUNKS;
+        const u32x4 raw = *reinterpret_cast<const u32x4*>(qp + min(4 * kk + g, CHUNKS - 1) * EPC + 8 * e);
+        qf[kk][e] = __builtin_bit_cast(vec8, in ? raw : u32x4{0u, 0u, 0u, 0u});
       }
   }
 
   struct Tile {
-    u32x4 k[NB][KC];
-    u32x4 v[DT];
-    float ks[PB], vs[PB];  // scales of unit g
-    uint32_t ok;           // unit g: bit h = its block h has a valid id
-  };
-  struct Ids {
-    int k[PB], v[PB];
+    u32x4 k[NG][KC];
+    VP v[NV][DT];
+    f32x2 sc;      // 8-bit: scales of K and V of entry (lane * entries / 64)
+    uint32_t bad;  // bit e: the block of entry e is outside the cache (wave-uniform)
   };
   const char* kbase = (const char*)a.key_cache + (int64_t)kvh * a.kv_head_stride * ES;
   const char* vbase = (const char*)a.value_cache + (int64_t)kvh * a.kv_head_stride * ES;
   const int64_t blk_bytes = a.kv_block_stride * ES;
+  const uint32_t k_lane = PB == 1 ? g * (BLK * 16) + c * 16 : g * (BLK * 16) + (c & 7) * 16;
+  const uint32_t v_lane = c * (BLK * ES) + (Q8 ? 0 : (PB == 1 ? 4 * g : 4 * (g & 1)) * ES);
 
-  // a unit without visible tokens is replaced by the last one of the sequence: its own blocks may
-  // have been given away already
-  auto unit_of = [&](int t, int u) {
-    const int unit = t * 4 + u;
-    const int tok = unit * U;
-    const bool seen = tok < R.len && (tok + U > R.lo || tok < R.sink_end);
-    return seen ? unit : (R.len - 1) / U;
-  };
-  auto load_ids = [&](Ids& id, int i) {
-    const int t = R.tile(i);
-    const int uk = unit_of(t, c >> 2), uv = unit_of(t, g);
+  auto issue = [&](Tile& t, int tile, const Ids& id) {
+    // An entry (8 or 16 tokens) without visible tokens may name anything, its block can have been
+    // given away: the entry before it is read instead, or the first visible one.
+    constexpr int NE = NG * PB, ET = 16 / PB;
+    int use[NE], at = 0, seen = 0;
 #pragma unroll
-    for (int h = 0; h < PB; ++h) {
-      // the second half of the last unit may lie past the sequence's blocks: the last block again
-      id.k[h] = table[min(uk * U + h * BLK, R.len - 1) / BLK];
-      id.v[h] = table[min(uv * U + h * BLK, R.len - 1) / BLK];
-    }
-  };
-  auto issue = [&](Tile& t, const Ids& id, int i) {
-    const int tile = R.tile(i);
-    const int uk = unit_of(tile, c >> 2), uv = unit_of(tile, g);
-    t.ok = 0;
-    const char *kp[PB], *vp[PB];
-#pragma unroll
-    for (int h = 0; h < PB; ++h) {
-      const bool k_ok = (unsigned)id.k[h] < (uint64_t)a.num_blocks, v_ok = (unsigned)id.v[h] < (uint64_t)a.num_blocks;
-      t.ok |= v_ok ? 1u << h : 0u;
-      const int64_t kb = k_ok ? id.k[h] : 0, vb = v_ok ? id.v[h] : 0;
-      // K: [chunk][BLK tokens][16 bytes]; V: [d][BLK tokens]
-      kp[h] = kbase + kb * blk_bytes + (PB == 1 ? uk * U % BLK : 0) * 16 + (c & 3) * 16 + g * (BLK * 16);
-      vp[h] = vbase + vb * blk_bytes + (PB == 1 ? uv * U % BLK : 0) * ES + c * (BLK * ES);
-      if constexpr (Q8) {
-        const float* sc = a.kv_scales + (vb * a.num_kv_heads + kvh) * 2;
-        t.ks[h] = sc[0];
-        t.vs[h] = sc[1];
-      }
+    for (int e = 0; e < NE; ++e) {
+      const int tok = (tile * NE + e) * ET;
+      int v = (int)(tok < R.len) & ((int)(tok + ET > R.lo) | (int)(tok < R.sink_end));
+      // (the block that the step appends to is needed whole, also where a window hides its first half)
+      if constexpr (STEP) v |= (int)(tok / BLK == (R.len - 1) / BLK);
+      at = v ? id.e[e] : at;
+      seen |= v << e;
+      use[e] = at;
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const char* p = PB == 1 ? kp[0] + b * 64 : kp[b / (NB / PB)] + (b % (NB / PB)) * 64;
+    for (int e = NE - 1; e >= 0; --e) {
+      at = (seen >> e & 1) ? id.e[e] : at;
+      use[e] = (seen & ((2 << e) - 1)) ? use[e] : at;
+    }
+    t.bad = 0;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const bool out_of_cache = (uint32_t)use[e] >= (uint64_t)a.num_blocks;
+      t.bad |= out_of_cache ? (uint32_t)(seen & (1 << e)) : 0u;
+      use[e] = out_of_cache ? 0 : use[e];
+    }
+    diag |= t.bad ? PE_DIAG_BLOCK_ID : 0;
+#pragma unroll
+    for (int h = 0; h < NG; ++h) {
+      const int sub = BLK == 32 ? (tile * NG + h) & 1 : 0;
+      int64_t ko;  // bytes from kbase
+      if constexpr (PB == 1) ko = use[h] * blk_bytes + sub * 256;
+      else ko = (c < 8 ? use[2 * h] : use[2 * h + PB - 1]) * blk_bytes;
+      const char* kl = kbase + ko + k_lane;
 #pragma unroll
       for (int kk = 0; kk < KC; ++kk) {
-        t.k[b][kk] = u32x4{0u, 0u, 0u, 0u};
+        t.k[h][kk] = u32x4{0u, 0u, 0u, 0u};
         if (4 * kk + 3 < CHUNKS || 4 * kk + g < CHUNKS)
-          t.k[b][kk] = *reinterpret_cast<const u32x4*>(p + kk * (4 * BLK * 16));
+          t.k[h][kk] = win_load<STREAM>(reinterpret_cast<const u32x4*>(kl + kk * (4 * BLK * 16)));
       }
     }
+    if constexpr (Q8) {
+      // the lane's group: g.  Scales: a vector load in line with K and V (a scalar one would be waited
+      // for together with the next tile's ids), each lane the entry that lane * entries / 64 names.
+      const char* vl[PB];
+      int mine[PB];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      t.v[dt] = u32x4{0u, 0u, 0u, 0u};
-      if (16 * dt + 15 < D || 16 * dt + c < D) {
+      for (int p = 0; p < PB; ++p) {
+        const int lo = g == 0 ? use[p] : use[PB + p], hi = g == 2 ? use[(NG - 2) * PB + p] : use[(NG - 1) * PB + p];
+        mine[p] = g < 2 ? lo : hi;
+        vl[p] = vbase + mine[p] * blk_bytes + (BLK == 32 ? (g & 1) * 16 : 0) + v_lane;
+      }
+      const int scaled = PB == 1 || c < 8 ? mine[0] : mine[PB - 1];
+      t.sc = *reinterpret_cast<const f32x2*>(a.kv_scales + ((int64_t)scaled * a.num_kv_heads + kvh) * 2);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
         if constexpr (PB == 1) {
-          t.v[dt] = *reinterpret_cast<const u32x4*>(vp[0] + dt * (16 * BLK * ES));
+          t.v[0][dt] = win_load<STREAM>(reinterpret_cast<const u32x4*>(vl[0] + dt * (16 * BLK)));
         } else {
-          const u32x2 lo = *reinterpret_cast<const u32x2*>(vp[0] + dt * (16 * BLK * ES));
-          const u32x2 hi = *reinterpret_cast<const u32x2*>(vp[1] + dt * (16 * BLK * ES));
-          t.v[dt] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+          const u32x2 lo = win_load<STREAM>(reinterpret_cast<const u32x2*>(vl[0] + dt * (16 * BLK)));
+          const u32x2 hi = win_load<STREAM>(reinterpret_cast<const u32x2*>(vl[PB - 1] + dt * (16 * BLK)));
+          t.v[0][dt] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < NG; ++h) {
+        int64_t vo;
+        if constexpr (PB == 1) vo = use[h] * blk_bytes + (BLK == 32 ? ((tile * NG + h) & 1) * 32 : 0);
+        else vo = (g < 2 ? use[2 * h] : use[2 * h + PB - 1]) * blk_bytes;
+        const char* vl = vbase + vo + v_lane;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          t.v[h][dt] = VP{};
+          if (16 * dt + 15 < D || 16 * dt + c < D)
+            t.v[h][dt] = win_load<STREAM>(reinterpret_cast<const VP*>(vl + dt * (16 * BLK * ES)));
         }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);  // the requests stay in front of the arithmetic that follows
   };
 
   float m_run = WIN_NEG, l_run = 0.f;  // log2 units; l_run: this lane's tokens only
@@ -203,128 +267,283 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_window_kernel(const WinAr
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto compute = [&](Tile& t, int i) {
-    const int tile = R.tile(i);
+  auto compute = [&](Tile& t, int tile) {
     const int t0 = tile * TOK;
-    f32x4 s[NB];
+    f32x4 s[NG];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < NG; ++h) {
+      s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < KC; ++kk) {
-        const u32x4 w = t.k[b][kk];
+        const u32x4 k = t.k[h][kk];
         if constexpr (Q8) {
-          s[b] = TR::mfma16(codes8<T, C>(w[0], w[1]), qf[kk][0], s[b]);
-          s[b] = TR::mfma16(codes8<T, C>(w[2], w[3]), qf[kk][1], s[b]);
+          s[h] = TR::mfma16(codes8<T, C>(k[0], k[1]), qf[kk][0], s[h]);
+          s[h] = TR::mfma16(codes8<T, C>(k[2], k[3]), qf[kk][1], s[h]);
         } else {
-          s[b] = TR::mfma16(__builtin_bit_cast(vec8, w), qf[kk][0], s[b]);
+          s[h] = TR::mfma16(__builtin_bit_cast(vec8, k), qf[kk][0], s[h]);
         }
       }
     }
+    // the lane's tokens lie in block 0 or 1 of a group: 8-token blocks switch at g = 2
+    const int mine = PB == 1 ? 0 : g >> 1;
     const bool inside = t0 + TOK <= R.len && (t0 >= R.lo || t0 + TOK <= R.sink_end);
-    const bool good = __builtin_amdgcn_ballot_w64(t.ok != (1u << PB) - 1u) == 0;
-    const bool masked = !(inside && good);  // wave-uniform
-    const int tok0 = t0 + g * U;
-    auto hidden = [&](int e) {  // token e of the lane's unit
-      const int tok = tok0 + e;
-      const bool block_ok = (t.ok >> (PB == 1 ? 0 : e / (U / PB))) & 1u;
-      return !(tok < R.len && (tok >= R.lo || tok < R.sink_end) && block_ok);
+    const bool masked = !inside || t.bad != 0;  // wave-uniform
+    // token 4g + r of group h
+    auto shown = [&](int h, int r) {
+      return visible(t0 + 16 * h + 4 * g + r) & (int)(~t.bad >> (h * PB + mine) & 1u);
     };
+    float ks[NG], vs[NG];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const float f = Q8 ? a.scale_log2 * t.ks[b / (NB / PB)] : a.scale_log2;
-      s[b] *= f;
+    for (int h = 0; h < NG; ++h) {
+      ks[h] = a.scale_log2;
+      vs[h] = 1.f;
+      if constexpr (Q8) {
+        // entry e lies in lanes e * 64 / entries ...
+        auto scale_of = [&](int e, int i) {
+          return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.sc[i]), e * (16 / PB)));
+        };
+        ks[h] *= mine == 0 ? scale_of(h * PB, 0) : scale_of(h * PB + PB - 1, 0);
+        vs[h] = mine == 0 ? scale_of(h * PB, 1) : scale_of(h * PB + PB - 1, 1);
+      }
+      s[h] *= ks[h];
     }
     if (masked) {
-      if (!good && lane % 16 == 0 && t.ok != (1u << PB) - 1u) {
-        // report an id outside the cache only where one of its tokens would have been visible
-        for (int e = 0; e < U; ++e) {
-          const int tok = tok0 + e;
-          if (tok < R.len && (tok >= R.lo || tok < R.sink_end) && hidden(e))
-            atomicOr(&window_diag_word, (unsigned)PE_DIAG_BLOCK_ID);
-        }
-      }
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int h = 0; h < NG; ++h)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[b][r] = hidden(4 * b + r) ? -INFINITY : s[b][r];
+        for (int r = 0; r < 4; ++r) s[h][r] = shown(h, r) ? s[h][r] : -INFINITY;
     }
-    float mx[PB], lv[PB];
+    float mx[NG];
 #pragma unroll
-    for (int h = 0; h < PB; ++h) {
-      mx[h] = -INFINITY;
+    for (int h = 0; h < NG; ++h) mx[h] = fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3]));
+    float top = mx[0];
 #pragma unroll
-      for (int b = h * (NB / PB); b < (h + 1) * (NB / PB); ++b)
-        mx[h] = fmaxf(mx[h], fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])));
-    }
-    const float m_new = fmaxf(m_run, win_max_groups(PB == 1 ? mx[0] : fmaxf(mx[0], mx[PB - 1])));
+    for (int h = 1; h < NG; ++h) top = fmaxf(top, mx[h]);
+    const float m_new = fmaxf(m_run, win_max_groups(top));
     float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
     l_run *= alpha;
-    float wf[PB];  // factor of the lane's probabilities in front of V
     if constexpr (WREF) {
-      float y = -INFINITY;
+      float y = -INFINITY, lv[NG];
 #pragma unroll
-      for (int h = 0; h < PB; ++h) {
-        lv[h] = __builtin_amdgcn_logf(t.vs[h]);  // log2; -inf for a block of zeros
+      for (int h = 0; h < NG; ++h) {
+        lv[h] = __builtin_amdgcn_logf(vs[h]);  // log2; -inf for a block of zeros
         y = fmaxf(y, mx[h] + lv[h]);
       }
       const float w_new = fmaxf(w_run, win_max_groups(y));
       alpha = __builtin_amdgcn_exp2f(w_run - w_new);
 #pragma unroll
-      for (int h = 0; h < PB; ++h) wf[h] = __builtin_amdgcn_exp2f(lv[h] + (m_new - w_new));
+      for (int h = 0; h < NG; ++h) vs[h] = __builtin_amdgcn_exp2f(lv[h] + (m_new - w_new));
       w_run = w_new;
-    } else {
-#pragma unroll
-      for (int h = 0; h < PB; ++h) wf[h] = Q8 ? t.vs[h] : 1.f;
     }
     m_run = m_new;
-    vec8 pf[NP];
+    float w[NG][4];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int h = 0; h < NG; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(s[b][r] - m_new);
+        const float p = __builtin_amdgcn_exp2f(s[h][r] - m_new);
         l_run += p;
-        float w = Q8 ? p * wf[b / (NB / PB)] : p;
-        if (Q8 && masked) w = hidden(4 * b + r) ? 0.f : w;  // the scale may be anything there
-        pf[b >> 1][(b & 1) * 4 + r] = (T)w;
+        w[h][r] = Q8 ? p * vs[h] : p;
       }
-    // hidden slots may hold anything (NaN included): their values become zero
-    if (masked) {
-      u32x4 keep;
+    if (Q8 && masked) {  // a hidden token's scale may be anything
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t mk = 0;
+      for (int h = 0; h < NG; ++h)
 #pragma unroll
-        for (int e = 0; e < 4 / ES; ++e)
-          mk |= hidden(w * (4 / ES) + e) ? 0u : (ES == 1 ? 0xffu : 0xffffu) << (8 * ES * e);
-        keep[w] = mk;
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) t.v[dt] &= keep;
+        for (int r = 0; r < 4; ++r) w[h][r] = shown(h, r) ? w[h][r] : 0.f;
     }
+    vec8 pf[NG / 2];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      acc[dt] *= alpha;
-      const u32x4 w = t.v[dt];
-      if constexpr (Q8) {
-        acc[dt] = TR::mfma16(codes8<T, C>(w[0], w[1]), pf[0], acc[dt]);
-        acc[dt] = TR::mfma16(codes8<T, C>(w[2], w[3]), pf[NP - 1], acc[dt]);
-      } else {
-        acc[dt] = TR::mfma16(__builtin_bit_cast(vec8, w), pf[0], acc[dt]);
+    for (int h = 0; h < NG; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) pf[h >> 1][(h & 1) * 4 + r] = (T)w[h][r];
+    // hidden slots may hold anything (NaN included): their values become zero
+    if constexpr (Q8) {
+      if (masked) {
+        u32x4 keep;
+#pragma unroll
+        for (int w4 = 0; w4 < 4; ++w4) {
+          uint32_t mk = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int v = visible(t0 + 16 * g + 4 * w4 + e) & (int)(~t.bad >> (g * PB + (PB == 1 ? 0 : w4 >> 1)) & 1u);
+            mk |= v ? 0xffu << (8 * e) : 0u;
+          }
+          keep[w4] = mk;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) t.v[0][dt] &= keep;
+      }
+      // P to the lane group of its tokens: register j of lane group h <- register h of lane group j
+      uint32_t pt[4][2];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const u32x4 two = __builtin_bit_cast(u32x4, pf[h >> 1]);
+        pt[h][0] = two[(h & 1) * 2];
+        pt[h][1] = two[(h & 1) * 2 + 1];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const auto x = __builtin_amdgcn_permlane32_swap(pt[h][e], pt[h + 2][e], false, false);
+          pt[h][e] = x[0];
+          pt[h + 2][e] = x[1];
+        }
+#pragma unroll
+        for (int h = 0; h < 4; h += 2) {
+          const auto x = __builtin_amdgcn_permlane16_swap(pt[h][e], pt[h + 1][e], false, false);
+          pt[h][e] = x[0];
+          pt[h + 1][e] = x[1];
+        }
+      }
+      const vec8 p0 = __builtin_bit_cast(vec8, u32x4{pt[0][0], pt[0][1], pt[1][0], pt[1][1]});
+      const vec8 p1 = __builtin_bit_cast(vec8, u32x4{pt[2][0], pt[2][1], pt[3][0], pt[3][1]});
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const u32x4 v = t.v[0][dt];
+        acc[dt] *= alpha;
+        acc[dt] = TR::mfma16(codes8<T, C>(v[0], v[1]), p0, acc[dt]);
+        acc[dt] = TR::mfma16(codes8<T, C>(v[2], v[3]), p1, acc[dt]);
+      }
+    } else {
+      if (masked) {
+#pragma unroll
+        for (int h = 0; h < NG; ++h) {
+          const u32x2 keep = {(shown(h, 0) ? 0xffffu : 0u) | (shown(h, 1) ? 0xffff0000u : 0u),
+                              (shown(h, 2) ? 0xffffu : 0u) | (shown(h, 3) ? 0xffff0000u : 0u)};
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) t.v[h][dt] &= keep;
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const u32x2 lo = t.v[0][dt], hi = t.v[NV - 1][dt];
+        acc[dt] *= alpha;
+        acc[dt] = TR::mfma16(__builtin_bit_cast(vec8, u32x4{lo[0], lo[1], hi[0], hi[1]}), pf[0], acc[dt]);
       }
     }
   };
 
-  {
-    Tile t0;
-    Ids id;
-    for (int i = i_begin + wave; i < i_end; i += WAVES) {
-      load_ids(id, i);
-      issue(t0, id, i);
-      compute(t0, i);
+  // ---- STEP: the new row into the cache and the last tile ---------------------------------------
+  // Returns whether the tile has to be read again: a row larger than everything before it changes the
+  // older codes of its block, in memory (rare).
+  auto append = [&](Tile& t, int tile) -> bool {
+    if constexpr (STEP) {
+      constexpr int NE = NG * PB, ET = 16 / PB;
+      const int pos = R.len - 1, o = pos % BLK;  // position, slot in its block
+      const int hn = (pos >> 4) - tile * NG, en = pos / ET - tile * NE;
+      if (t.bad >> en & 1) return false;  // its block is outside the cache
+      const int64_t blk = table[pos / BLK];
+      const T* krow = (const T*)a.new_key + (int64_t)seq * a.new_k_stride + (int64_t)kvh * D;
+      const T* vrow = (const T*)a.new_value + (int64_t)seq * a.new_v_stride + (int64_t)kvh * D;
+      u32x4 kx[KC][2];  // the lane's chunks of the key row: elements 16 * (4 kk + g) ..
+      uint16_t vx[DT];  // the lane's elements of the value row: 16 dt + c
+#pragma unroll
+      for (int kk = 0; kk < KC; ++kk) {
+        const int ch = min(4 * kk + g, CHUNKS - 1);
+        kx[kk][0] = *reinterpret_cast<const u32x4*>(krow + ch * 16);
+        kx[kk][1] = *reinterpret_cast<const u32x4*>(krow + ch * 16 + 8);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vx[dt] = reinterpret_cast<const uint16_t*>(vrow)[16 * dt + c];
+      uint32_t ka = 0, va = 0;
+#pragma unroll
+      for (int kk = 0; kk < KC; ++kk)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t w = kx[kk][e >> 2][e & 3];
+          ka = max(ka, max(finite_bits<T>(w & 0xffffu), finite_bits<T>(w >> 16)));
+        }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) va = max(va, finite_bits<T>(vx[dt]));
+#pragma unroll
+      for (int x = 16; x <= 32; x <<= 1) ka = max(ka, (uint32_t)__shfl_xor((int)ka, x));
+#pragma unroll
+      for (int x = 1; x <= 8; x <<= 1) va = max(va, (uint32_t)__shfl_xor((int)va, x));
+      auto old_scale = [&](int i) {
+        return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.sc[i]), en * (64 / NE)));
+      };
+      const float ks_old = o ? old_scale(0) : 0.f, vs_old = o ? old_scale(1) : 0.f;
+      const float ks = fmaxf(ks_old, pow2_scale<C>(bits_value<T>(ka)));
+      const float vs = fmaxf(vs_old, pow2_scale<C>(bits_value<T>(va)));
+      const float ki = ks > 0.f ? 1.f / ks : 1.f, vi = vs > 0.f ? 1.f / vs : 1.f;
+      char* kw = const_cast<char*>(kbase) + blk * blk_bytes;
+      char* vw = const_cast<char*>(vbase) + blk * blk_bytes;
+      const bool k_grew = ks_old > 0.f && ks > ks_old, v_grew = vs_old > 0.f && vs > vs_old;
+      const bool grew = __builtin_amdgcn_ballot_w64(k_grew || v_grew) != 0;  // wave-uniform
+      if (grew) {
+        if (k_grew)
+          for (int it = lane; it < CHUNKS * o * 4; it += 64)
+            reencode_word<C>(reinterpret_cast<uint32_t*>(kw + it / (o * 4) * (BLK * 16)) + it % (o * 4), ks_old * ki);
+        if (v_grew)
+          for (int it = lane; it < D * o; it += 64)
+            reencode_byte<C>(reinterpret_cast<uint8_t*>(vw + it / o * BLK + it % o), vs_old * vi);
+      }
+      // K: the row is token pos & 15 of group hn
+#pragma unroll
+      for (int h = 0; h < NG; ++h) {
+        if (h != hn) continue;  // wave-uniform
+        const bool here = c == (pos & 15);
+#pragma unroll
+        for (int kk = 0; kk < KC; ++kk) {
+          u32x4 code;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const u32x4 x = kx[kk][w >> 1];
+            const uint32_t lo = x[(w & 1) * 2], hi = x[(w & 1) * 2 + 1];
+            code[w] = encode4<C>(bits_value<T>(lo & 0xffffu) * ki, bits_value<T>(lo >> 16) * ki,
+                                 bits_value<T>(hi & 0xffffu) * ki, bits_value<T>(hi >> 16) * ki);
+          }
+          if (here && 4 * kk + g < CHUNKS) {
+            t.k[h][kk] = code;
+            *reinterpret_cast<u32x4*>(kw + ((4 * kk + g) * BLK + o) * 16) = code;
+          }
+        }
+      }
+      // V: the lanes of group g hold its 16 tokens of row 16 dt + c; the row goes to byte pos & 15
+      const bool mine = BLK == 32 ? (g >> 1) == (hn >> 1) : g == hn;
+      if (g == hn) {
+        const uint32_t sh = 8 * (pos & 3);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint32_t code = encode4<C>(bits_value<T>(vx[dt]) * vi, 0.f, 0.f, 0.f) & 255u;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t now = t.v[0][dt][w];
+            t.v[0][dt][w] = ((pos & 15) >> 2) == w ? (now & ~(0xffu << sh)) | (code << sh) : now;
+          }
+          reinterpret_cast<uint8_t*>(vw)[(16 * dt + c) * BLK + o] = (uint8_t)code;
+        }
+      }
+      const bool scaled = BLK == 8 ? lane * NE / 64 == en : mine;
+      if (scaled) t.sc = f32x2{ks, vs};
+      if (lane == 0) {
+        float* sc = const_cast<float*>(a.kv_scales) + (blk * a.num_kv_heads + kvh) * 2;
+        *reinterpret_cast<f32x2*>(sc) = f32x2{ks, vs};
+      }
+      if (grew) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "agent");  // the stores before the next loads
+      return grew;
     }
+    return false;
+  };
+
+  // ---- the wave's tiles ------------------------------------------------------------------------
+  // (A second tile in flight gains nothing: 167.8 against 167.6 us on 945 MB, 21.5 against 20.3 on
+  // 64 x 776 tokens; the waves of a CU hold 128 KiB in flight as it is.  A tile number past the end
+  // only names table entries, which load_ids keeps inside the row.)
+  for (int i = i0; i < R.tiles; i += step) {
+    Tile t;
+    issue(t, at(i), ids);
+    if constexpr (STEP) {
+      if (i == early) {
+        if (raw_len > most) diag |= PE_DIAG_APPEND_MISMATCH;
+        else if (append(t, at(i))) issue(t, at(i), ids);
+      }
+    }
+    ids = load_ids(at(i + step));
+    compute(t, at(i));
   }
+  if (diag != 0 && lane == 0) atomicOr(&window_diag_word, diag);
 
   // ---- join the lane groups' sums, then the waves through LDS ---------------------------------
   l_run += __shfl_xor(l_run, 16);
@@ -367,7 +586,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_window_kernel(const WinAr
     if (a.num_splits == 1) {
       ((T*)a.out)[((int64_t)seq * a.num_heads + head) * D + d] = (T)(l == 0.f ? 0.f : o / l);
     } else {
-      float* w = a.ws + (((int64_t)split * gridDim.z + seq) * a.num_heads + head) * win_ws_stride(D);
+      float* w = a.ws + (((int64_t)split * num_seqs + seq) * a.num_heads + head) * win_ws_stride(D);
       if (d == 0) {
         w[0] = m_tot;
         w[1] = l;
@@ -377,41 +596,88 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_window_kernel(const WinAr
   }
 }
 
-template <typename T, typename C, int D, int WAVES, int BLK>
+// Joins the splits of one (query head, sequence): all partials (at most MS) are read at once.
+template <typename T, int MS>
+__global__ __launch_bounds__(256) void paged_window_merge_kernel(T* __restrict__ out, const float* __restrict__ ws,
+                                                                  int num_heads, int head_size, int num_splits) {
+  const int head = blockIdx.x, seq = blockIdx.y, d = threadIdx.x;
+  const int64_t split_stride = (int64_t)gridDim.y * num_heads * win_ws_stride(head_size);
+  const float* w = ws + ((int64_t)seq * num_heads + head) * win_ws_stride(head_size);
+  float m[MS], l[MS], o[MS];
+#pragma unroll
+  for (int s = 0; s < MS; ++s) {
+    // (past the last split: the last one again, with a weight of 0)
+    const float* p = w + min(s, num_splits - 1) * split_stride;
+    m[s] = p[0];
+    l[s] = s < num_splits ? p[1] : 0.f;
+    o[s] = s < num_splits ? p[2 + min(d, head_size - 1)] : 0.f;
+  }
+  float m_tot = m[0], lt = 0.f, ot = 0.f;
+#pragma unroll
+  for (int s = 1; s < MS; ++s) m_tot = fmaxf(m_tot, m[s]);
+#pragma unroll
+  for (int s = 0; s < MS; ++s) {
+    const float f = __builtin_amdgcn_exp2f(m[s] - m_tot);
+    lt += f * l[s];
+    ot += f * o[s];
+  }
+  if (d < head_size) out[((int64_t)seq * num_heads + head) * head_size + d] = (T)(lt == 0.f ? 0.f : ot / lt);
+}
+
+template <typename T, typename C, int D, int WAVES, int BLK, bool STEP>
 inline void launch_window(const WinArgs& a, dim3 grid, hipStream_t st) {
   constexpr int DT = (D + 15) / 16;
   const int gqa = a.num_heads / a.num_kv_heads, heads = gqa < 16 ? gqa : 16;
   const size_t lds = ((size_t)WAVES * heads * (16 * DT + 4) + 2 * WAVES * 16) * 4;
   if (lds > 64 * 1024)
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_window_kernel<T, C, D, WAVES, BLK>),
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_window_kernel<T, C, D, WAVES, BLK, STEP>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL((paged_window_kernel<T, C, D, WAVES, BLK>), grid, dim3(WAVES * 64), lds, st, a);
+  hipLaunchKernelGGL((paged_window_kernel<T, C, D, WAVES, BLK, STEP>), grid, dim3(WAVES * 64), lds, st, a);
+  if (a.num_splits == 1) return;
+  const dim3 mg((unsigned)a.num_heads, grid.z), mb(D <= 64 ? 64 : D <= 128 ? 128 : 256);
+#define PE_WIN_MERGE(MS) \
+  hipLaunchKernelGGL((paged_window_merge_kernel<T, MS>), mg, mb, 0, st, (T*)a.out, a.ws, a.num_heads, D, a.num_splits)
+  if (a.num_splits <= 4) PE_WIN_MERGE(4);
+  else if (a.num_splits <= 8) PE_WIN_MERGE(8);
+  else if (a.num_splits <= 16) PE_WIN_MERGE(16);
+  else PE_WIN_MERGE(32);
+#undef PE_WIN_MERGE
 }
 
-template <typename T, typename C, int D>
-inline int dispatch_window_block(const WinArgs& a, int block_size, dim3 grid, hipStream_t st) {
+template <typename T, typename C, int D, bool STEP>
+inline int dispatch_window_block(const WinArgs& a, int block_size, int waves, dim3 grid, hipStream_t st) {
+  if (waves == 8) switch (block_size) {
+    case 8: launch_window<T, C, D, 8, 8, STEP>(a, grid, st); return PE_OK;
+    case 16: launch_window<T, C, D, 8, 16, STEP>(a, grid, st); return PE_OK;
+    case 32: launch_window<T, C, D, 8, 32, STEP>(a, grid, st); return PE_OK;
+  }
   switch (block_size) {
-    case 8: launch_window<T, C, D, 4, 8>(a, grid, st); return PE_OK;
-    case 16: launch_window<T, C, D, 4, 16>(a, grid, st); return PE_OK;
-    case 32: launch_window<T, C, D, 4, 32>(a, grid, st); return PE_OK;
+    case 8: launch_window<T, C, D, 4, 8, STEP>(a, grid, st); return PE_OK;
+    case 16: launch_window<T, C, D, 4, 16, STEP>(a, grid, st); return PE_OK;
+    case 32: launch_window<T, C, D, 4, 32, STEP>(a, grid, st); return PE_OK;
   }
   return fail(PE_ERR_UNSUPPORTED, "paged_decode_window: block size %d (8, 16 or 32)", block_size);
 }
 
 // head sizes of one translation unit; the 16-bit cache also has 120
-template <typename T, typename C>
-inline int dispatch_window(const WinArgs& a, int head_size, int block_size, dim3 grid, hipStream_t st) {
+template <typename T, typename C, bool STEP = false>
+inline int dispatch_window(const WinArgs& a, int head_size, int block_size, int waves, dim3 grid, hipStream_t st) {
   switch (head_size) {
-    case 32: return dispatch_window_block<T, C, 32>(a, block_size, grid, st);
-    case 64: return dispatch_window_block<T, C, 64>(a, block_size, grid, st);
-    case 80: return dispatch_window_block<T, C, 80>(a, block_size, grid, st);
-    case 96: return dispatch_window_block<T, C, 96>(a, block_size, grid, st);
-    case 112: return dispatch_window_block<T, C, 112>(a, block_size, grid, st);
-    case 128: return dispatch_window_block<T, C, 128>(a, block_size, grid, st);
-    case 192: return dispatch_window_block<T, C, 192>(a, block_size, grid, st);
-    case 256: return dispatch_window_block<T, C, 256>(a, block_size, grid, st);
+    case 32: return dispatch_window_block<T, C, 32, STEP>(a, block_size, waves, grid, st);
+    case 64: return dispatch_window_block<T, C, 64, STEP>(a, block_size, waves, grid, st);
+    case 128: return dispatch_window_block<T, C, 128, STEP>(a, block_size, waves, grid, st);
+    case 80: return dispatch_window_block<T, C, 80, STEP>(a, block_size, waves, grid, st);
+    case 96: return dispatch_window_block<T, C, 96, STEP>(a, block_size, waves, grid, st);
+    case 112: return dispatch_window_block<T, C, 112, STEP>(a, block_size, waves, grid, st);
+    // (larger heads have no registers left for the append: pe_decode_step_8bit writes their row first)
+    case 192:
+      if constexpr (!STEP) return dispatch_window_block<T, C, 192, STEP>(a, block_size, waves, grid, st);
+      break;
+    case 256:
+      if constexpr (!STEP) return dispatch_window_block<T, C, 256, STEP>(a, block_size, waves, grid, st);
+      break;
     case 120:
-      if constexpr (__is_same(T, C)) return dispatch_window_block<T, C, 120>(a, block_size, grid, st);
+      if constexpr (__is_same(T, C)) return dispatch_window_block<T, C, 120, STEP>(a, block_size, waves, grid, st);
   }
   return fail(PE_ERR_UNSUPPORTED, "paged_decode_window: head size %d is not built", head_size);
 }
