@@ -8,88 +8,101 @@
 // rounds those that become subnormal.
 //
 // One workgroup owns one (sequence, block, KV head): the maximum over the block's new rows, the
-// re-expression of its older codes and the scale are decided in one place, without atomics.
-// Bound: HBM (2 bytes read, 1 written per element); a decode step (one row per sequence) by the
-// chain of dependent loads lengths -> table -> scale / rows.
+// re-expression of its older codes and the scale are decided in one place, without atomics.  A wave
+// takes four tokens x 16 chunks of 16 bytes (lane group g: token 4k + g), so rows come in 256-byte runs
+// and the codes of a value row's four tokens meet in one dword by two row swaps and four byte permutes;
+// the block goes through LDS in the cache's layout and is stored 16 bytes per lane.  The KV heads of a
+// block are dispatched side by side: their pieces of a token's row lie side by side.
+// Bound: HBM (2 bytes read, 1 written per element): 4 x 8192 rows of 8 x 128, int8, 42.5 us (4.3 TB/s;
+// a copy reaches 4.9); a decode step (one
+// row per sequence) by the chain of dependent loads lengths -> rows / table -> scale: 64 x 8 x 128, 4.6 us.
 #include "kv8.h"
 
 namespace pe {
 
-constexpr int W8_THREADS = 256;
+constexpr int w8_groups(int head_size) { return (head_size / 8 + 15) / 16; }            // chunk groups of a row
+constexpr int w8_items(int head_size, int block_size) { return block_size / 4 * w8_groups(head_size); }
+constexpr int w8_waves(int head_size, int block_size) {
+  return w8_items(head_size, block_size) < 4 ? w8_items(head_size, block_size) : 4;
+}
 
 static __device__ unsigned int cache8_diag_word;
 
-// I: 16-byte chunks of a block's new K (or V) rows per thread = block_size * head_size / 8 / 256
-template <typename T, typename F, int I>
-__global__ __launch_bounds__(W8_THREADS) void cache8_write_kernel(
+template <typename T, typename F, int D, int BLK>
+__global__ __launch_bounds__(64 * w8_waves(D, BLK)) void cache8_write_kernel(
     const T* __restrict__ key, const T* __restrict__ value, uint8_t* __restrict__ key_cache,
     uint8_t* __restrict__ value_cache, float* __restrict__ kv_scales,
     const int32_t* __restrict__ block_tables, const int32_t* __restrict__ seq_lens,
     const int32_t* __restrict__ cu_q, int64_t num_tokens, int64_t key_stride, int64_t value_stride,
-    int num_kv_heads, int head_size, int block_size, int64_t num_blocks, int table_width,
-    int64_t kv_block_stride, int64_t kv_head_stride) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t w8_smem[];  // K image, V image of the block
-  __shared__ uint32_t red[2][W8_THREADS / 64];
-  const int seq = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+    int num_kv_heads, int64_t num_blocks, int table_width, int64_t kv_block_stride, int64_t kv_head_stride) {
+  constexpr int CH = D / 8;                  // 16-byte chunks of a row
+  constexpr int WAVES = w8_waves(D, BLK), THREADS = 64 * WAVES;
+  constexpr int CG = w8_groups(D);
+  constexpr int I = w8_items(D, BLK) / WAVES;  // (token quad, chunk group) pairs per wave
+  // value image: rows of BLK bytes, 16 more after every 8 rows (spreads the dword writes over the banks)
+  constexpr int V_IMG = D * BLK + D / 8 * 16;
+  __shared__ __attribute__((aligned(16))) uint8_t k_img[D * BLK];
+  __shared__ __attribute__((aligned(16))) uint8_t v_img[V_IMG];
+  __shared__ uint32_t red[2][WAVES];
+  const int h = blockIdx.x, seq = blockIdx.z, tid = threadIdx.x;
+  const int lane = tid & 63, wave = tid >> 6, g = lane >> 4, c16 = lane & 15;
   const int64_t row0 = cu_q ? cu_q[seq] : seq;
   const int64_t row1 = cu_q ? cu_q[seq + 1] : seq + 1;
   const int64_t len = seq_lens[seq];
   if (len <= 0 || row1 <= row0) return;
   // lengths that do not fit together (more new rows than the sequence's length, rows past the
   // tensors, a length past the table row): nothing of the sequence is written
-  if (row0 < 0 || row1 > num_tokens || row1 - row0 > len || len > (int64_t)table_width * block_size) {
+  if (row0 < 0 || row1 > num_tokens || row1 - row0 > len || len > (int64_t)table_width * BLK) {
     if (tid == 0) atomicOr(&cache8_diag_word, (unsigned)PE_DIAG_APPEND_MISMATCH);
     return;
   }
   const int64_t ctx = len - (row1 - row0);
-  const int CH = head_size >> 3;  // 16-byte chunks of a row
-  uint8_t* const k_img = w8_smem;
-  uint8_t* const v_img = w8_smem + block_size * head_size;
 
-  for (int64_t j = ctx / block_size + blockIdx.x; j * block_size < len; j += gridDim.x) {
-    const int64_t p0 = j * block_size > ctx ? j * block_size : ctx;
-    const int64_t p1 = (j + 1) * block_size < len ? (j + 1) * block_size : len;
-    const int o0 = (int)(p0 - j * block_size), m = (int)(p1 - p0);  // first offset, new rows
-    const int64_t blk = block_tables[(int64_t)seq * table_width + j];
-    if (blk < 0 || blk >= num_blocks) {  // workgroup-uniform
-      if (tid == 0) atomicOr(&cache8_diag_word, (unsigned)PE_DIAG_BLOCK_ID);
-      continue;
-    }
-    float* sc = kv_scales + (blk * num_kv_heads + h) * 2;
-    const float ks_old = o0 ? sc[0] : 0.f, vs_old = o0 ? sc[1] : 0.f;
+  for (int64_t j = ctx / BLK + blockIdx.y; j * BLK < len; j += gridDim.y) {
+    const int o0 = (int)(j * BLK > ctx ? 0 : ctx - j * BLK);                  // first new slot
+    const int o1 = (int)((j + 1) * BLK < len ? (int64_t)BLK : len - j * BLK);  // behind the last one
+    const int blk = block_tables[(int64_t)seq * table_width + j];
 
     // ---- the new rows, kept in registers; the largest finite magnitudes ----------------------
     u32x4 kr[I], vr[I];
     uint32_t ka = 0, va = 0;
-    const int64_t r0 = row0 + (p0 - ctx);
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const int it = tid + i * W8_THREADS;
+      const int item = wave * I + i, slot = item / CG * 4 + g, c = item % CG * 16 + c16;
       kr[i] = vr[i] = u32x4{0u, 0u, 0u, 0u};
-      if (it < m * CH) {
-        const int64_t row = r0 + it / CH;
-        const int c = it % CH;
-        kr[i] = *reinterpret_cast<const u32x4*>(key + row * key_stride + (int64_t)h * head_size + c * 8);
-        vr[i] = *reinterpret_cast<const u32x4*>(value + row * value_stride + (int64_t)h * head_size + c * 8);
+      if (slot >= o0 && slot < o1 && c < CH) {
+        const int64_t row = row0 + (j * BLK + slot - ctx);
+        kr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(key + row * key_stride + (int64_t)h * D + c * 8));
+        vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(value + row * value_stride + (int64_t)h * D + c * 8));
       }
+    }
+    if (blk < 0 || blk >= num_blocks) {  // workgroup-uniform
+      if (tid == 0) atomicOr(&cache8_diag_word, (unsigned)PE_DIAG_BLOCK_ID);
+      continue;
+    }
+    float* sc = kv_scales + ((int64_t)blk * num_kv_heads + h) * 2;
+    const float ks_old = o0 ? sc[0] : 0.f, vs_old = o0 ? sc[1] : 0.f;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         ka = max(ka, max(finite_bits<T>(kr[i][e] & 0xffffu), finite_bits<T>(kr[i][e] >> 16)));
         va = max(va, max(finite_bits<T>(vr[i][e] & 0xffffu), finite_bits<T>(vr[i][e] >> 16)));
       }
-    }
+    // (both are 16-bit magnitudes: one word carries the two maxima through the wave)
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) {
-      ka = max(ka, (uint32_t)__shfl_xor((int)ka, x));
-      va = max(va, (uint32_t)__shfl_xor((int)va, x));
+      const uint32_t other = (uint32_t)__shfl_xor((int)(ka | va << 16), x);
+      ka = max(ka, other & 0xffffu);
+      va = max(va, other >> 16);
     }
-    if ((tid & 63) == 0) {
-      red[0][tid >> 6] = ka;
-      red[1][tid >> 6] = va;
+    if (lane == 0) {
+      red[0][wave] = ka;
+      red[1][wave] = va;
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < W8_THREADS / 64; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       ka = max(ka, red[0][w]);
       va = max(va, red[1][w]);
     }
@@ -102,28 +115,21 @@ __global__ __launch_bounds__(W8_THREADS) void cache8_write_kernel(
     uint8_t* vb = value_cache + blk * kv_block_stride + (int64_t)h * kv_head_stride;
     // ---- older codes at the grown scale (rare: a row larger than everything before it) --------
     if (ks_old > 0.f && ks > ks_old) {
-      const float f = ks_old * ki;
-      for (int it = tid; it < (head_size >> 4) * o0 * 4; it += W8_THREADS) {
-        const int c = it / (o0 * 4), w = it % (o0 * 4);
-        reencode_word<F>(reinterpret_cast<uint32_t*>(kb + c * block_size * 16) + w, f);
-      }
+      for (int it = tid; it < D / 16 * o0 * 4; it += THREADS)
+        reencode_word<F>(reinterpret_cast<uint32_t*>(kb + it / (o0 * 4) * (BLK * 16)) + it % (o0 * 4), ks_old * ki);
     }
     if (vs_old > 0.f && vs > vs_old) {
-      const float f = vs_old * vi;
-      for (int it = tid; it < head_size * o0; it += W8_THREADS)
-        reencode_byte<F>(vb + (it / o0) * block_size + it % o0, f);
+      for (int it = tid; it < D * o0; it += THREADS) reencode_byte<F>(vb + it / o0 * BLK + it % o0, vs_old * vi);
     }
     if (tid == 0) {
       sc[0] = ks;
       sc[1] = vs;
     }
     // ---- the new codes ------------------------------------------------------------------------
-    const bool whole = m == block_size;
+    const bool whole = o0 == 0 && o1 == BLK;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const int it = tid + i * W8_THREADS;
-      if (it >= m * CH) continue;
-      const int off = o0 + it / CH, c = it % CH;
+      const int item = wave * I + i, slot = item / CG * 4 + g, c = item % CG * 16 + c16;
       auto enc = [&](const u32x4& r, float inv) {
         float f[8];
 #pragma unroll
@@ -134,24 +140,35 @@ __global__ __launch_bounds__(W8_THREADS) void cache8_write_kernel(
         return u32x2{encode4<F>(f[0], f[1], f[2], f[3]), encode4<F>(f[4], f[5], f[6], f[7])};
       };
       const u32x2 kc = enc(kr[i], ki), vc = enc(vr[i], vi);
-      const int k_at = ((c >> 1) * block_size + off) * 16 + (c & 1) * 8;
+      const int k_at = ((c >> 1) * BLK + slot) * 16 + (c & 1) * 8;
       if (whole) {
-        *reinterpret_cast<u32x2*>(k_img + k_at) = kc;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          v_img[(c * 8 + e) * block_size + off] = (uint8_t)(vc[e >> 2] >> (8 * (e & 3)));
-      } else {
+        // 8 elements x 4 tokens of a chunk, spread over the four lane groups -> two dwords per lane:
+        // elements 2g and 2g + 1, four tokens each
+        const auto x = __builtin_amdgcn_permlane32_swap(vc[0], vc[1], false, false);
+        // groups 0, 1: elements 0-3 of tokens g, g + 2; groups 2, 3: elements 4-7 of tokens g - 2, g
+        const uint32_t p = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), q = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+        const auto y = __builtin_amdgcn_permlane16_swap(p, q, false, false);
+        const uint32_t d0 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), d1 = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u);
+        if (c < CH) {
+          *reinterpret_cast<u32x2*>(k_img + k_at) = kc;
+          uint32_t* v = reinterpret_cast<uint32_t*>(v_img + (c * 8 + 2 * g) * BLK + c * 16 + item / CG * 4);
+          v[0] = d0;
+          v[BLK / 4] = d1;
+        }
+      } else if (slot >= o0 && slot < o1 && c < CH) {
         *reinterpret_cast<u32x2*>(kb + k_at) = kc;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          vb[(c * 8 + e) * block_size + off] = (uint8_t)(vc[e >> 2] >> (8 * (e & 3)));
+        for (int e = 0; e < 8; ++e) vb[(c * 8 + e) * BLK + slot] = (uint8_t)(vc[e >> 2] >> (8 * (e & 3)));
       }
     }
     __syncthreads();  // images complete; the next block's maxima may overwrite `red`
     if (whole) {
-      for (int it = tid; it < block_size * head_size / 16; it += W8_THREADS) {
-        reinterpret_cast<u32x4*>(kb)[it] = reinterpret_cast<const u32x4*>(k_img)[it];
-        reinterpret_cast<u32x4*>(vb)[it] = reinterpret_cast<const u32x4*>(v_img)[it];
+      for (int it = tid; it < D * BLK / 16; it += THREADS) {
+        // (8 value rows are BLK / 2 pieces of 16 bytes.  Rows in and codes out pass the caches once: with the
+        //  non-temporal hint 42.5 us, without 44.7)
+        __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(k_img)[it], reinterpret_cast<u32x4*>(kb) + it);
+        __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(v_img)[it + it / (BLK / 2)],
+                                    reinterpret_cast<u32x4*>(vb) + it);
       }
       __syncthreads();
     }
@@ -191,28 +208,32 @@ extern "C" int pe_reshape_and_cache_8bit(
   PE_REQUIRE(key_stride % 8 == 0 && value_stride % 8 == 0 && ((uintptr_t)key | (uintptr_t)value) % 16 == 0,
              PE_ERR_INVALID_ARG, "reshape_and_cache_8bit: key/value rows must be 16-byte aligned");
   PE_REQUIRE(num_seqs <= 65535 && num_kv_heads <= 65535, PE_ERR_UNSUPPORTED, "reshape_and_cache_8bit: grid too large");
-  const int most = max_q_len == 1 ? 1 : (max_q_len + block_size - 2) / block_size + 1;  // blocks a sequence touches
-  dim3 grid((unsigned)most, (unsigned)num_kv_heads, (unsigned)num_seqs);
-  const size_t lds = 2 * (size_t)block_size * head_size;
+  // blocks a sequence touches (the kernel goes on in strides of the grid where there are more)
+  const int64_t most = max_q_len == 1 ? 1 : ((int64_t)max_q_len + block_size - 2) / block_size + 1;
+  dim3 grid((unsigned)num_kv_heads, (unsigned)(most < 65535 ? most : 65535), (unsigned)num_seqs);
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define PE_W8(T, F, I)                                                                               \
-  hipLaunchKernelGGL((cache8_write_kernel<T, F, I>), grid, dim3(W8_THREADS), lds, st, (const T*)key, \
-                     (const T*)value, (uint8_t*)key_cache, (uint8_t*)value_cache, kv_scales,         \
-                     block_tables, seq_lens, cu_q, num_tokens, key_stride, value_stride,             \
-                     num_kv_heads, head_size, block_size, num_blocks, max_num_blocks_per_seq,        \
-                     kv_block_stride, kv_head_stride)
-#define PE_W8_I(T, F)                                                     \
-  do {                                                                    \
-    const int chunks = block_size * head_size / 8;                        \
-    if (chunks <= W8_THREADS) PE_W8(T, F, 1);                             \
-    else if (chunks <= 2 * W8_THREADS) PE_W8(T, F, 2);                    \
-    else PE_W8(T, F, 4);                                                  \
-  } while (0)
+#define PE_W8(T, F, D, BLK)                                                                               \
+  hipLaunchKernelGGL((cache8_write_kernel<T, F, D, BLK>), grid, dim3(64 * w8_waves(D, BLK)), 0, st,       \
+                     (const T*)key, (const T*)value, (uint8_t*)key_cache, (uint8_t*)value_cache,          \
+                     kv_scales, block_tables, seq_lens, cu_q, num_tokens, key_stride, value_stride,       \
+                     num_kv_heads, num_blocks, max_num_blocks_per_seq, kv_block_stride, kv_head_stride)
+#define PE_W8_BLK(T, F, D)                  \
+  case D:                                   \
+    if (block_size == 8) PE_W8(T, F, D, 8); \
+    else if (block_size == 16) PE_W8(T, F, D, 16); \
+    else PE_W8(T, F, D, 32);                \
+    break
+#define PE_W8_D(T, F)                                                                                     \
+  switch (head_size) {                                                                                    \
+    PE_W8_BLK(T, F, 32); PE_W8_BLK(T, F, 64); PE_W8_BLK(T, F, 80); PE_W8_BLK(T, F, 96);                   \
+    PE_W8_BLK(T, F, 112); PE_W8_BLK(T, F, 128); PE_W8_BLK(T, F, 192); PE_W8_BLK(T, F, 256);               \
+  }
   PE_DISPATCH_16(dtype, T, {
-    if (kv_format == PE_KV_FP8_E4M3) PE_W8_I(T, Fp8);
-    else PE_W8_I(T, Int8);
+    if (kv_format == PE_KV_FP8_E4M3) PE_W8_D(T, Fp8)
+    else PE_W8_D(T, Int8)
   });
-#undef PE_W8_I
+#undef PE_W8_D
+#undef PE_W8_BLK
 #undef PE_W8
   return check_launch("reshape_and_cache_8bit");
 }
