@@ -459,7 +459,10 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     const int count = ns + max(0, n_tiles - tw);
     auto tile_at = [&](int i) { return i < ns ? i : tw + i - ns; };
     if (count > 0) {
+      // the first two tiles together: where the first holds a few sinks, its arithmetic would not cover
+      // the way of the second
       stage(tile_at(0), 0);
+      if (count > 1) stage(tile_at(1), 1);
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -469,7 +472,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
       const int wrow1 = wrow0 + WROWS - 1;  // last row of the wave
       for (int i = 0; i < count; ++i) {
         const int tile = tile_at(i), buf = i & 1;
-        if (i + 1 < count) stage(tile_at(i + 1), buf ^ 1);
+        if (i > 0 && i + 1 < count) stage(tile_at(i + 1), buf ^ 1);
         const int k0 = tile * BN, k1 = k0 + BN - 1;
         // wave-uniform: some row sees some key / every row sees every key
         const bool some = k0 <= wrow1 && (window == 0 || k1 > wrow0 - window || k0 < sinks);
