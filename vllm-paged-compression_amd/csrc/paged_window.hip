@@ -32,34 +32,37 @@ int window_diag_fetch(unsigned int* out, int reset) {
 }
 
 // Workgroup width (waves) and number of splits over the keys of a launch.  A split costs a merge launch
-// (about 2.5 us); a wave takes its tiles (16 KiB at head size 128) one memory round trip after the
-// other, so a launch that cannot fill the chip wants one tile per wave.  Measured on MI355X
-// (graph-replayed, us; waves/splits; workgroups without splits x tiles of a sequence):
+// (about 2.5 us of GPU time, 2 us of host time where launches are not replayed from a graph); a wave
+// takes its tiles (16 KiB at head size 128) one memory round trip after the other, so a launch that
+// cannot fill the chip wants them on many waves.  Measured on MI355X (us graph-replayed, | issued one by
+// one; waves/splits; workgroups without splits x tiles of a sequence):
 //   512 x 112 (64 x 8192 tokens, 8 bit): 4/1 154, 4/2 156, 8/1 172; 512 x 32: 42 / 45 / 49; 512 x 13: 19 / 24 / 22
 //   512 x 33 (16 bit): 4/1 45, 4/2 49, 8/1 52; 512 x 64: 75 / 80 / 86; 2048 x 4: 22 / 41 / 43
 //   256 x 13: 4/1 12.5, 8/1 13.1, 4/2 15.0; 192 x 65 (head 64): 4/1 29, 4/2 22, 4/4 21, 8/1 21
 //   128 x 128: 4/1 58, 4/2 43, 4/4 43, 8/1 55; 32 x 512: 4/4 60, 4/8 43, 8/8 50
-//    64 x 65: 4/4 16.7, 4/6 17.6, 4/8 15.7, 8/1 22; 64 x 49: 4/4 14.5, 4/6 15.2, 4/8 15.9, 8/1 19; 64 x 25: 4/4 9.4, 8/1 9.4
-//     8 x 65: 4/8 11.1, 8/8 8.9, 8/9 8.2; 8 x 25: 4/4 8.3, 4/7 6.8, 8/1 8.0; 12 x 13: 4/1 8.2, 4/4 6.7, 8/1 7.5
+//    64 x 65: 4/4 16.7, 4/8 15.7, 8/1 22; 64 x 49: 4/4 14.5, 4/8 15.9, 8/1 19; 64 x 25: 4/4 9.4, 8/1 9.4
+//    64 x 13: 12/1 8.4 | 7.8, 4/4 8.7 | 8.5, 4/1 10; 32 x 13: 12/1 7.5 | 7.3, 4/4 8.4 | 8.4
+//    12 x 13 (head 64): 16/1 7.4 | 7.1, 4/4 6.7 | 8.4, 4/1 8.5; 8 x 7: 12/1 6.5 | 6.2, 4/2 7.5 | 8.4
+//     8 x 32: 12/3 8.6 | 8.5, 4/8 8.5 | 8.5, 12/1 11; 8 x 65: 8/9 8.2, 4/8 11; 6 x 24 (head 64): 16/1 7.7 | 7.4
 struct WinShape {
   int waves, splits;
 };
-static WinShape window_shape(int num_seqs, int num_heads, int num_kv_heads, int max_seq_len, int window,
-                             int sinks, int kv_format) {
+static WinShape window_shape(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_seq_len,
+                             int window, int sinks, int kv_format, bool step) {
   const int gqa = num_heads / num_kv_heads;
   const int64_t wgs = (int64_t)num_seqs * num_kv_heads * ((gqa + 15) / 16);
   const int tok = kv_format == PE_KV_SAME ? 32 : 64;
   const int64_t seen = window > 0 && (int64_t)window + sinks < max_seq_len ? (int64_t)window + sinks : max_seq_len;
   // (a window and its sinks may each begin and end inside a tile)
   const int64_t tiles = (seen + tok - 1) / tok + (window > 0 && seen < max_seq_len ? 1 + (sinks > 0) : 0);
+  const int wide = win_wide(head_size, step);
   WinShape s{4, 1};
-  if (tiles <= 4) return s;
-  if (wgs >= 256) return s;  // the chip is full
-  if (wgs * tiles <= 1024) {  // one tile per wave
-    if (tiles > 32) s.waves = 8;
+  if (tiles <= 4 || wgs >= 256) return s;  // nothing to share out, or the chip is full
+  if (wgs * tiles <= 4352 && tiles <= 2 * wide) {  // one launch, at most two tiles per wave
+    s.waves = wide;
+  } else if (wgs * tiles <= 1024) {  // one tile per wave
+    if (tiles > 32) s.waves = wide;
     s.splits = (int)((tiles + s.waves - 1) / s.waves);
-  } else if (wgs * tiles <= 4352 && tiles <= 32) {
-    s.waves = 8;
   } else {  // bound by bandwidth: a workgroup per CU
     s.splits = (int)((256 + wgs - 1) / wgs);
   }
@@ -92,7 +95,10 @@ static int window_decode(const char* who, void* out, const void* query, const vo
   const int gqa = num_heads / num_kv_heads, groups = (gqa + 15) / 16;
   PE_REQUIRE(num_seqs <= 65535 && (int64_t)num_kv_heads * groups <= 65535, PE_ERR_UNSUPPORTED,
              "%s: grid too large", who);
-  const WinShape shape = window_shape(num_seqs, num_heads, num_kv_heads, max_seq_len, window, sinks, kv_format);
+  // The row is written by a launch of its own where several workgroups read the block that it joins (more
+  // than 16 query heads on a KV head) and where the kernel has no registers left for it
+  const bool step = new_key != nullptr && groups == 1 && head_size <= 128;
+  const WinShape shape = window_shape(num_seqs, num_heads, num_kv_heads, head_size, max_seq_len, window, sinks, kv_format, step);
   const int splits = shape.splits, waves = shape.waves;
   if (splits > 1) {
     const int64_t need = (int64_t)splits * num_seqs * num_heads * win_ws_stride(head_size) * 4;
@@ -105,9 +111,6 @@ static int window_decode(const char* who, void* out, const void* query, const vo
                   new_key, new_value, new_k_stride, new_v_stride};
   const dim3 grid((unsigned)splits, (unsigned)(num_kv_heads * groups), (unsigned)num_seqs);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // The row is written by a launch of its own where several workgroups read the block that it joins (more
-  // than 16 query heads on a KV head) and where the kernel has no registers left for it
-  const bool step = new_key != nullptr && groups == 1 && head_size <= 128;
   if (new_key != nullptr && !step) {
     if (int rc = pe_reshape_and_cache_8bit(new_key, new_value, const_cast<void*>(key_cache),
                                            const_cast<void*>(value_cache), const_cast<float*>(kv_scales), block_tables,
@@ -135,9 +138,13 @@ int64_t pe_paged_window_workspace_bytes(int num_seqs, int num_heads, int num_kv_
                                         int max_seq_len, int sliding_window, int num_sinks, int kv_format) {
   using namespace pe;
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0) return 0;
-  const int splits =
-      window_shape(num_seqs, num_heads, num_kv_heads, max_seq_len, sliding_window, num_sinks, kv_format).splits;
-  return splits <= 1 ? 0 : (int64_t)splits * num_seqs * num_heads * win_ws_stride(head_size) * 4;
+  int64_t splits = 1;  // of the attention alone and of the step
+  for (bool step : {false, true}) {
+    const WinShape w = window_shape(num_seqs, num_heads, num_kv_heads, head_size, max_seq_len, sliding_window,
+                                    num_sinks, kv_format, step);
+    splits = splits < w.splits ? w.splits : splits;
+  }
+  return splits <= 1 ? 0 : splits * num_seqs * num_heads * win_ws_stride(head_size) * 4;
 }
 
 int pe_paged_decode_window(void* out, const void* query, const void* key_cache, const void* value_cache,

@@ -44,6 +44,11 @@ struct WinArgs {
   int64_t new_k_stride, new_v_stride;
 };
 
+// waves of the wide workgroup: as many as the registers of a head size allow
+constexpr int win_wide(int head_size, bool step) {
+  return step ? (head_size <= 64 ? 12 : 8) : head_size <= 64 ? 16 : head_size <= 128 ? 12 : 8;
+}
+
 __host__ __device__ inline int64_t win_ws_stride(int head_size) { return head_size + 2; }
 
 template <bool NT, typename V>
@@ -89,7 +94,7 @@ __host__ __device__ inline WinRange win_range(int len, int window, int sinks) {
 // (and, where the block's scale grows, the re-expressed older codes) into the tile's registers and into
 // the cache, and goes on with the attention.  No other wave of the launch touches the block.
 template <typename T, typename C, int D, int WAVES, int BLK, bool STEP>
-__global__ __launch_bounds__(WAVES * 64, 2) void paged_window_kernel(const WinArgs a) {
+__global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_window_kernel(const WinArgs a) {
   using TR = Traits<T>;
   using vec8 = typename TR::vec8;
   constexpr bool Q8 = !__is_same(C, T);
@@ -646,10 +651,11 @@ inline void launch_window(const WinArgs& a, dim3 grid, hipStream_t st) {
 
 template <typename T, typename C, int D, bool STEP>
 inline int dispatch_window_block(const WinArgs& a, int block_size, int waves, dim3 grid, hipStream_t st) {
-  if (waves == 8) switch (block_size) {
-    case 8: launch_window<T, C, D, 8, 8, STEP>(a, grid, st); return PE_OK;
-    case 16: launch_window<T, C, D, 8, 16, STEP>(a, grid, st); return PE_OK;
-    case 32: launch_window<T, C, D, 8, 32, STEP>(a, grid, st); return PE_OK;
+  constexpr int WIDE = win_wide(D, STEP);
+  if (waves == WIDE) switch (block_size) {
+    case 8: launch_window<T, C, D, WIDE, 8, STEP>(a, grid, st); return PE_OK;
+    case 16: launch_window<T, C, D, WIDE, 16, STEP>(a, grid, st); return PE_OK;
+    case 32: launch_window<T, C, D, WIDE, 32, STEP>(a, grid, st); return PE_OK;
   }
   switch (block_size) {
     case 8: launch_window<T, C, D, 4, 8, STEP>(a, grid, st); return PE_OK;
