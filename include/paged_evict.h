@@ -663,15 +663,16 @@ int pe_swap_blocks(const void* src, void* dst, const int64_t* block_mapping_host
  * Prefill attention with a sliding window and sink tokens: pe_prefill_causal whose query i attends
  * kv rows j <= min(i, Lkv-1) with sliding_window == 0, or j > i - sliding_window, or j < num_sinks; a
  * query that sees no row gets zeros.  bf16 / f16, head sizes 32, 64, 80, 96, 112, 120, 128, 192,
- * 256, scale > 0.  max_q_len sizes the grid: rows of a request past it are not computed.  A NaN or
- * an infinity in k or v reaches the queries that see its row, no other (such a tile costs much
+ * 256, scale > 0.  max_q_len sizes the grid: rows of a request past it are not computed.  num_q_rows /
+ * num_kv_rows: rows that q (out) and k / v have; a request that cu_q or cu_kv places past them is cut.
+ * A NaN or an infinity in k or v reaches the queries that see its row, no other (such rows cost much
  * more time).
  * ---------------------------------------------------------------------------------- */
 int pe_prefill_window(void* out, const void* q, const void* k, const void* v, const int32_t* cu_q,
-                      const int32_t* cu_kv, int num_seqs, int max_q_len, int num_heads,
-                      int num_kv_heads, int head_size, int64_t q_stride, int64_t k_stride,
-                      int64_t v_stride, int64_t out_stride, float scale, int sliding_window,
-                      int num_sinks, int dtype, void* stream);
+                      const int32_t* cu_kv, int num_seqs, int max_q_len, int64_t num_q_rows,
+                      int64_t num_kv_rows, int num_heads, int num_kv_heads, int head_size,
+                      int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t out_stride,
+                      float scale, int sliding_window, int num_sinks, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------
  * 8-bit paged cache.  Element = code * scale; codes e4m3 (largest value 448) or int8 (-127 ..

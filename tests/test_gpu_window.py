@@ -135,6 +135,17 @@ def test_prefill_window_fewer_or_more_kv_rows(ops, sinks):
         assert (got[110:200] == 0).all() and (got[250:270] == 0).all()
 
 
+def test_prefill_window_prefix_sums_past_the_rows(ops):
+    """Prefix sums that reach past the rows of q or k are cut to them (never read or written past)."""
+    g = torch.Generator().manual_seed(16)
+    q, k, v = (rows(g, 90, h, 64, torch.bfloat16) for h in (4, 2, 2))
+    cu = torch.tensor([0, 40, 90], dtype=torch.int32).cuda()
+    far = torch.tensor([0, 40, 200], dtype=torch.int32).cuda()
+    want = ops.prefill_window(q.cuda(), k.cuda(), v.cuda(), cu, cu, 50, 0.125, 20, 1)
+    for a, b in ((far, far), (cu, far), (far, cu)):
+        assert torch.equal(want, ops.prefill_window(q.cuda(), k.cuda(), v.cuda(), a, b, 160, 0.125, 20, 1))
+
+
 def test_prefill_window_equals_causal_without_a_window(ops):
     g = torch.Generator().manual_seed(7)
     lens = [300, 41]

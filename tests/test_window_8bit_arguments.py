@@ -166,7 +166,7 @@ def test_c_entry_points_refuse_before_the_device():
     said(lib, window(bs=4), 2, b"block size")
 
     def prefill(D=64, scale=0.1, dtype=2, w=4, n=10, stride=256, S=1):
-        return lib.pe_prefill_window(P, P, P, P, P, P, S, n, 4, 2, D, stride, stride, stride, stride, scale, w, 0, dtype, None)
+        return lib.pe_prefill_window(P, P, P, P, P, P, S, n, 99, 99, 4, 2, D, stride, stride, stride, stride, scale, w, 0, dtype, None)
     assert prefill(S=0) == 0 and prefill(n=0) == 0
     said(lib, prefill(D=72), 2, b"head size")
     said(lib, prefill(scale=0.0), 2, b"scale")

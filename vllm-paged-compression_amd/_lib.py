@@ -109,7 +109,7 @@ SIGNATURES = {
                                c_void_p]),
     "pe_swap_blocks": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p]),
     "pe_prefill_window": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                                  c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64,
+                                  c_int, c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64,
                                   c_float, c_int, c_int, c_int, c_void_p]),
     "pe_reshape_and_cache_8bit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                           c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int,

@@ -8,7 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -157,17 +157,20 @@ void check_decode(const char* what, const at::Tensor& out, const at::Tensor& q, 
   REQ(window >= 0 && sinks >= 0, PyExc_ValueError, "%s: sliding_window and num_sinks must not be negative", what);
 }
 
+struct WithoutGil {  // (restored before an exception reaches the caller)
+  PyThreadState* state = PyEval_SaveThread();
+  ~WithoutGil() { PyEval_RestoreThread(state); }
+};
+
 // runs `fn` (stream) -> status with device `dev` current
 template <typename F>
 void launch(const char* what, int dev, F&& fn) {
-  hipStream_t st = c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream();
   int rc;
-  Py_BEGIN_ALLOW_THREADS;
-  const int cur = (int)c10::hip::current_device();
-  if (cur != dev) c10::hip::set_device((c10::DeviceIndex)dev);
-  rc = fn((void*)st);
-  if (cur != dev) c10::hip::set_device((c10::DeviceIndex)cur);
-  Py_END_ALLOW_THREADS;
+  {
+    const WithoutGil free;
+    const c10::hip::HIPGuard guard((c10::DeviceIndex)dev);
+    rc = fn((void*)c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream());
+  }
   REQ(rc == 0, PyExc_RuntimeError, "paged_evict %s failed (status %d): %s", what, rc, pe_last_error());
 }
 
@@ -344,7 +347,7 @@ PyObject* prefill_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
       launch(what, dev, [&](void* st) {
         return pe_prefill_window(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                  (const int32_t*)cu_q.data_ptr(), (const int32_t*)cu_kv.data_ptr(),
-                                 (int)cu_q.size(0) - 1, max_q, (int)Hq, (int)H, (int)D, row_stride(q), row_stride(k),
+                                 (int)cu_q.size(0) - 1, max_q, q.size(0), k.size(0), (int)Hq, (int)H, (int)D, row_stride(q), row_stride(k),
                                  row_stride(v), row_stride(out), (float)scale, window, sinks, row_dtype(q), st);
       });
     }

@@ -117,7 +117,8 @@ extern "C" int pe_prefill_causal(void* out, const void* q, const void* k, const 
           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);                                   \
     hipLaunchKernelGGL((prefill_mfma_kernel<T, HS, NR, WAVES, WPE>), grid, dim3(WAVES * 64), lds,  \
                        st, (T*)out, (const T*)q, (const T*)k, (const T*)v, cu_q, cu_kv, num_heads, \
-                       num_kv_heads, head_size, q_stride, k_stride, v_stride, out_stride, sl2, 0, 0, 1); \
+                       num_kv_heads, head_size, q_stride, k_stride, v_stride, out_stride, sl2, 0, 0, 1, \
+                       0, 0);                                                                      \
   } while (0)
 #define PE_LAUNCH_PF_SHAPE(T, HS)                                                                  \
   do {                                                                                             \

@@ -81,8 +81,8 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     const T* __restrict__ v, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_kv,
     int num_heads, int num_kv_heads, int head_size, int64_t q_stride, int64_t k_stride,
     int64_t v_stride, int64_t out_stride, float scale_log2e, int window, int sinks,
-    int heads_per_wg) {
-  // window, sinks, heads_per_wg: WIN only
+    int heads_per_wg, int num_q_rows, int num_kv_rows) {
+  // window and what follows: WIN only
   using TR = Traits<T>;
   using vec8 = typename TR::vec8;
   constexpr int KS = D / 32;
@@ -124,8 +124,9 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int head = WIN ? (kvh * gqa + hg) * hpw + wave % hpw : kvh * gqa + hg;
   const int bm = WIN ? BM / hpw : BM;  // query rows per workgroup and head
-  const int q0 = cu_q[seq], lq = cu_q[seq + 1] - q0;
-  const int kv0 = cu_kv[seq], lkv = cu_kv[seq + 1] - kv0;
+  const int q0 = cu_q[seq], lq = (WIN ? min(cu_q[seq + 1], num_q_rows) : cu_q[seq + 1]) - q0;
+  const int kv0 = cu_kv[seq], lkv = (WIN ? min(cu_kv[seq + 1], num_kv_rows) : cu_kv[seq + 1]) - kv0;
+  if (WIN && ((q0 | kv0) < 0 || cu_q[seq + 1] < q0 || cu_kv[seq + 1] < kv0)) return;  // no prefix sums
   const int qt = (int)gridDim.z - 1 - (int)blockIdx.z;
   const int m0 = qt * bm;
   if (m0 >= lq) return;

@@ -4,15 +4,17 @@
 
 extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const void* v,
                                  const int32_t* cu_q, const int32_t* cu_kv, int num_seqs,
-                                 int max_q_len, int num_heads, int num_kv_heads, int head_size,
+                                 int max_q_len, int64_t num_q_rows, int64_t num_kv_rows,
+                                 int num_heads, int num_kv_heads, int head_size,
                                  int64_t q_stride, int64_t k_stride, int64_t v_stride,
                                  int64_t out_stride, float scale, int sliding_window, int num_sinks,
                                  int dtype, void* stream) {
   using namespace pe;
-  PE_REQUIRE(num_seqs >= 0 && max_q_len >= 0, PE_ERR_INVALID_ARG, "prefill_window: negative size");
+  PE_REQUIRE(num_seqs >= 0 && max_q_len >= 0 && num_q_rows >= 0 && num_kv_rows >= 0, PE_ERR_INVALID_ARG,
+             "prefill_window: negative size");
   PE_REQUIRE(sliding_window >= 0 && num_sinks >= 0, PE_ERR_INVALID_ARG,
              "prefill_window: sliding_window %d and num_sinks %d must not be negative", sliding_window, num_sinks);
-  if (num_seqs == 0 || max_q_len == 0) return PE_OK;
+  if (num_seqs == 0 || max_q_len == 0 || num_q_rows == 0) return PE_OK;
   PE_REQUIRE(out && q && k && v && cu_q && cu_kv, PE_ERR_INVALID_ARG, "prefill_window: null pointer");
   PE_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0, PE_ERR_INVALID_ARG,
              "prefill_window: num_heads %d must be a positive multiple of num_kv_heads %d", num_heads, num_kv_heads);
@@ -22,6 +24,9 @@ extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const 
   PE_REQUIRE(dtype == PE_BF16 || dtype == PE_F16, PE_ERR_UNSUPPORTED, "prefill_window: dtype %d (bf16 or f16)", dtype);
   // the maxima are kept in scaled units
   PE_REQUIRE(scale > 0.f && scale < INFINITY, PE_ERR_UNSUPPORTED, "prefill_window: scale must be positive and finite");
+  // (the prefix sums are int32: rows past 2^31 - 1 belong to no request)
+  if (num_q_rows > INT32_MAX) num_q_rows = INT32_MAX;
+  if (num_kv_rows > INT32_MAX) num_kv_rows = INT32_MAX;
   PE_REQUIRE(max_q_len <= (1 << 22) && num_seqs <= 65535 && num_heads <= 65535, PE_ERR_UNSUPPORTED,
              "prefill_window: grid too large");
   PE_REQUIRE(q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0 && out_stride % 8 == 0 && k_stride > 0 &&
@@ -60,7 +65,7 @@ extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const 
     hipLaunchKernelGGL((prefill_mfma_kernel<T, HS, NR, WAVES, WPE, true, BN>), grid, dim3(WAVES * 64),  \
                        lds, st, (T*)out, (const T*)q, (const T*)k, (const T*)v, cu_q, cu_kv, num_heads, \
                        num_kv_heads, head_size, q_stride, k_stride, v_stride, out_stride, sl2,          \
-                       sliding_window, num_sinks, hpw);                                                 \
+                       sliding_window, num_sinks, hpw, (int)num_q_rows, (int)num_kv_rows);              \
   } while (0)
   PE_DISPATCH_16(dtype, T, {
     if (head_size <= 64) PE_LAUNCH_PW(T, 64, 1, 4, 2, 64);
