@@ -13,9 +13,9 @@
 // and the codes of a value row's four tokens meet in one dword by two row swaps and four byte permutes;
 // the block goes through LDS in the cache's layout and is stored 16 bytes per lane.  The KV heads of a
 // block are dispatched side by side: their pieces of a token's row lie side by side.
-// Bound: HBM (2 bytes read, 1 written per element): 4 x 8192 rows of 8 x 128, int8, 42.5 us (4.3 TB/s;
-// a copy reaches 4.9); a decode step (one
-// row per sequence) by the chain of dependent loads lengths -> rows / table -> scale: 64 x 8 x 128, 4.6 us.
+// Bound: HBM (2 bytes read, 1 written per element): 4 x 8192 rows of 8 x 128, int8, 39 us (4.7 TB/s, a
+// copy's rate); a decode step (one row per sequence) by the chain of dependent loads lengths -> rows /
+// table -> scale: 64 x 8 x 128, 4.6 us.
 #include "kv8.h"
 
 namespace pe {

@@ -17,6 +17,10 @@
 //     left where it lies the loads are 4 bytes: 260 instead of 168 us on 945 MB.
 // 8-bit codes are converted to the query's type exactly; K's scale multiplies the f32 scores, V's
 // scale the probabilities.
+//
+// Bound: HBM.  64 sequences x 7168 tokens on average, 8 KV heads x 128, int8: 945 MB in 154 us, 6.1 TB/s; the
+// same loads without conversion and second matrix product 150.  64 x 1028 of 8192 tokens in 16 bits: 270 MB in
+// 45 us, 6.0 TB/s.  64 x 776 in e4m3: 90 MB in 18.5 us (4.3 us of start and merge, the rest at 6.3 TB/s).
 #pragma once
 #include <type_traits>
 

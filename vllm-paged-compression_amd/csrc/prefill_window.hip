@@ -37,17 +37,18 @@ extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const 
   if (num_sinks > (1 << 30)) num_sinks = 1 << 30;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const float sl2 = scale * 1.4426950408889634f;
-  // Tile shape: 16 x NR query rows per wave, 4 waves (8 at the 256 pitch), BN keys per tile.  The waves
-  // take the query heads of a KV head side by side (hpw of them).  Measured on MI355X (us per launch,
-  // 2 rows-tiles x 64 keys / 1 x 64 / 1 x 32; 32 query and 8 KV heads x 128, 4 sinks; window 0 = none):
-  //   8 x 1024 tokens, window 64: 58 / 63 / 44, 128: 58 / 69 / 52, 256: 67 / 81 / 65, 512: 80 / 100 / 86,
-  //   none: 89 / 110 / 99; 4 x 4096, window 64: 114 / 142 / 97, 256: 144 / 185 / 149, 1024: 289 / 368 / 338;
-  //   1 x 512, window 64: 12.0 / 8.7 / 8.7, none: 17.9 / 13.7 / 16.7;
-  //   12 heads x 64, 8 x 1024, window 64: 25 / 18 / 19, 256: 32 / 23 / 25, none: 33 / 28 / 34.
-  // So: head sizes up to 64, and launches that leave CUs idle, take the 1 x 64 shape (more, smaller
-  // workgroups; at 64 elements a key costs half the LDS reads); rows that see few
-  // keys the 1 x 32 shape, whose tiles waste less at the window's two ends; everything else 2 x 64,
-  // which reads each K/V fragment from LDS once for 32 rows.
+  // Tile shape: 16 x NR query rows per wave, 4 waves (8 at the 256 pitch), BN keys per tile; the waves
+  // take the query heads of a KV head side by side (hpw of them).  Measured on MI355X (us per launch over
+  // three sets of inputs; NR x BN = 2 x 64 / 1 x 64 / 1 x 32; 32 query and 8 KV heads x 128, 4 sinks; none
+  // = no window):
+  //   8 x 1024 tokens, window 64: 59 / 71 / 48, 128: 64 / 75 / 57, 256: 73 / 88 / 74, 384: 79 / 98 / 83,
+  //   none: 94 / 116 / 109; 4 x 4096, window 64: 112 / 138 / 95, 256: 151 / 187 / 150, 512: 203 / 249 / 227,
+  //   none: 567 / 717 / 696; 1 x 512, window 64: 11.9 / 8.4 / 8.2, 256: 16.2 / 11.2 / 12.3, none: 17.7 / 12.8 / 16.0;
+  //   12 heads x 64, 8 x 1024, window 64: 24 / 18 / 18, 256: 31 / 22 / 24, none: 32 / 27 / 33.
+  // So: head sizes up to 64, and launches that leave CUs idle, take the 1 x 64 shape (more and smaller
+  // workgroups; at 64 elements a key costs half the LDS reads); rows that see few keys the 1 x 32 shape, whose
+  // tiles waste less at the window's two ends; everything else 2 x 64, which reads each K/V fragment from
+  // LDS once for 32 rows.
   const int gqa = num_heads / num_kv_heads;
   const int64_t span = sliding_window > 0 ? (int64_t)sliding_window + num_sinks : max_q_len;
   const int64_t wgs = (int64_t)num_seqs * num_heads * ((max_q_len + 127) / 128);  // of 2 x 64
