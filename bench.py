@@ -616,7 +616,7 @@ def kernel_source_hash(files=("paged_decode.hip", "paged_decode_kernel.h", "pe_c
     return h.hexdigest()
 
 
-PREFILL_SOURCES = ("prefill.hip", "pe_common.h")
+PREFILL_SOURCES = ("prefill.hip", "prefill_kernel.h", "pe_common.h")
 
 
 def stored_prefill_busy(flops_per_launch: float):

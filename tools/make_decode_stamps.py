@@ -42,6 +42,7 @@ def main():
     try:
         obj = os.path.join(OUT, "decode_stamps.o")
         subprocess.check_call(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
+                               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                                "-I" + os.path.join(ROOT, "include"), "-c", src, "-o", obj])
         objs = [os.path.join(PKG, "build", f) for f in os.listdir(os.path.join(PKG, "build"))
                 if f.endswith(".o") and f != "paged_decode.o"]

@@ -24,6 +24,7 @@ def main():
         lib = os.path.join(OUT, f"libpe_{name}.so")
         obj = os.path.join(OUT, f"paged_decode_{name}.o")
         subprocess.check_call(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
+                               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                                "-I" + os.path.join(ROOT, "include"), *flags, "-c", SRC, "-o", obj,
                                "-Rpass-analysis=kernel-resource-usage"],
                               stderr=open(os.path.join(OUT, f"{name}.remarks"), "w"))

@@ -10,8 +10,22 @@ import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "vllm-paged-compression_amd")
-SRC = os.path.join(PKG, "csrc", "prefill.hip")
+CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(ROOT, "tools", "_exp")
+
+
+PV = "#pragma unroll\n    for (int k2 = 0; k2 < NS / 2; ++k2) pv_step(vt, k2, pf);\n"   # P.V of a whole tile
+
+
+def prefill_source():
+    """prefill.hip with the kernel template of prefill_kernel.h in place of its include."""
+    with open(os.path.join(CSRC, "prefill_kernel.h")) as f:
+        kernel = f.read().replace("#pragma once\n", "", 1)
+    with open(os.path.join(CSRC, "prefill.hip")) as f:
+        text = f.read()
+    include = '#include "prefill_kernel.h"\n'
+    assert include in text
+    return text.replace(include, kernel, 1)
 
 
 def variant(name, text):
@@ -40,8 +54,8 @@ def variant(name, text):
         text = variant("nobar", text)
     if name == "qk_nov":     # QK MFMAs and K reads only: no V reads, no softmax, no P.V, no staging, no barrier
         text = variant("qkonly", text)
-        a = text.index("    const int tq = c >> 2, tp = c & 3;")
-        b = text.index("  };\n\n  // ---- main loop")
+        a = text.index(PV)
+        b = a + len(PV)
         text = text[:a] + ("#pragma unroll\n    for (int sub = 0; sub < 4; ++sub)\n#pragma unroll\n"
                            "      for (int n = 0; n < NR; ++n) acc[sub][n] += s[sub][n];\n"
                            "    (void)pf;\n") + text[b:]
@@ -52,7 +66,7 @@ def variant(name, text):
                             "        dst[ks] = qf[0][(ks + sub) % KS];")
     if name == "qk_noread32":  # the same flops as qk_noread issued as 16 v_mfma_f32_32x32x16
         text = variant("qk_nov", text)
-        a = text.index("    f32x4 s[4][NR];")
+        a = text.index("    f32x4 s[NS][NR];")
         b = text.index("    // ---- mask, online softmax")
         text = text[:a] + """    f32x4 s[4][NR];
     f32x16 z[2];
@@ -78,8 +92,8 @@ def variant(name, text):
                             "s[sub][n][ks & 3] += (float)kf[sub & 1][ks][n];")
     if name == "v_noqk":     # V reads + P.V MFMAs only (P = ones), no K reads, no QK, no softmax, no staging, no barrier
         text = variant("nobar", text)
-        a = text.index("    f32x4 s[4][NR];")
-        b = text.index("    // ---- O^T += V^T.P^T")
+        a = text.index("    f32x4 s[NS][NR];")
+        b = text.index(PV)
         text = text[:a] + ("    vec8 pf[NR][2];\n#pragma unroll\n    for (int n = 0; n < NR; ++n) { pf[n][0] = ones; pf[n][1] = ones; }\n"
                            "    (void)n0; (void)kt;\n") + text[b:]
     return text
@@ -87,7 +101,7 @@ def variant(name, text):
 
 def main():
     os.makedirs(OUT, exist_ok=True)
-    base = open(SRC).read()
+    base = prefill_source()
     objs = [os.path.join(PKG, "build", f) for f in os.listdir(os.path.join(PKG, "build"))
             if f.endswith(".o") and f != "prefill.o"]
     for name in sys.argv[1:] or ["noload", "nobar", "nosoftmax", "novalu", "nopv"]:
@@ -100,6 +114,7 @@ def main():
             lib = os.path.join(OUT, f"libpe_{name}.so")
             obj = os.path.join(OUT, f"prefill_{name}.o")
             subprocess.check_call(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
+                                   "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                                    "-I" + os.path.join(ROOT, "include"), "-c", src, "-o", obj])
             subprocess.check_call(["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib, obj, *objs])
             os.remove(obj)

@@ -10,7 +10,7 @@
 //   pattern 2: V as eight 16-byte-per-lane loads (half a row each, lane groups 0/1 one block,
 //              2/3 the other) and K with the token order that layout of P needs (each load
 //              touches half of sixteen 128-byte lines)
-// Build and run: hipcc --offload-arch=gfx950 -O3 -o cu_pull_rate cu_pull_rate.hip && ./cu_pull_rate
+// Build and run: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o cu_pull_rate cu_pull_rate.hip && ./cu_pull_rate
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>

@@ -2,7 +2,7 @@
 // accumulators live in the AccVGPR half of the register file (so that the matrix instruction's
 // C/D traffic does not compete for the ports the vector instructions read)?  One workgroup of
 // 4 waves (one per SIMD) on one CU; shader clocks per group of 1 MFMA + KV vector instructions.
-// Build and run: hipcc --offload-arch=gfx950 -O3 -o mfma_agpr_overlap mfma_agpr_overlap.hip && ./mfma_agpr_overlap
+// Build and run: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o mfma_agpr_overlap mfma_agpr_overlap.hip && ./mfma_agpr_overlap
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>

@@ -10,7 +10,7 @@
 //   placement: consumer on the producer's XCD (workgroup id + 8) or on the next XCD (id + 1)
 //   load: idle chip, or every CU also running a loop that streams random 4 KiB slabs
 // Every spin is bounded; a pair that gives up is counted, not waited for.
-// Build and run: hipcc --offload-arch=gfx950 -O3 -o xwg_handoff xwg_handoff.hip && ./xwg_handoff
+// Build and run: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o xwg_handoff xwg_handoff.hip && ./xwg_handoff
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>

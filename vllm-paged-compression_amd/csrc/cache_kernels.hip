@@ -8,7 +8,7 @@
 // layout allows it.
 #include <atomic>
 
-#include "pe_common.h"
+#include "kv8.h"
 
 namespace pe {
 

@@ -7,6 +7,10 @@
 
 namespace pe {
 
+// diagnostic words behind pe_device_diagnostics (defined in paged_window.hip / cache_8bit.hip)
+int window_diag_fetch(unsigned int* out, int reset);
+int cache8_diag_fetch(unsigned int* out, int reset);
+
 struct Fp8 {  // e4m3: 1 sign, 4 exponent, 3 mantissa bits; 0x7f / 0xff are NaN, no infinities
   static constexpr float MAX = 448.f;
   // 448 = 1.75 * 2^8: a scale 2^k holds amax = m * 2^e (1 <= m < 2) when k >= e - 8 + (m > 1.75)

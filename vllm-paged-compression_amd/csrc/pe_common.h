@@ -55,13 +55,10 @@ struct EnvInt {
   }
 };
 
-// per-file diagnostic words behind pe_device_diagnostics (defined in paged_decode.hip / evict.hip /
-// paged_window.hip / cache_8bit.hip)
+// per-file diagnostic words behind pe_device_diagnostics (defined in paged_decode.hip / evict.hip)
 int decode_diag_fetch(unsigned int* out, int reset);
 int evict_diag_fetch(unsigned int* out, int reset);
 int state_diag_fetch(unsigned int* out, int reset);
-int window_diag_fetch(unsigned int* out, int reset);
-int cache8_diag_fetch(unsigned int* out, int reset);
 
 // ---- storage types ---------------------------------------------------------------
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
