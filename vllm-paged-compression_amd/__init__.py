@@ -3,6 +3,7 @@
 Layout
   csrc/                 HIP kernels + the extern "C" entry points (include/paged_evict.h)
   _lib.py               ctypes binding; no fallback when the shared library is missing
+  csrc/host_binding.cpp checks and launches of the 8-bit cache's and windowed operators
   ops.py                torch-level operators mirroring the reference's vllm._custom_ops
   paged_attn.py         PagedAttention static wrapper (mirror of vllm/attention/ops/paged_attn.py)
   config.py             PagedEvictConfig (mirror of vllm/config.py:933-991)
