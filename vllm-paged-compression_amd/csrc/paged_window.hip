@@ -34,13 +34,19 @@ int window_diag_fetch(unsigned int* out, int reset) {
 // Workgroup width (waves) and number of splits over the keys of a launch.  A split costs a merge launch
 // (about 2.5 us of GPU time, 2 us of host time where launches are not replayed from a graph); a wave
 // takes its tiles (16 KiB at head size 128) one memory round trip after the other, so a launch that
-// cannot fill the chip wants them on many waves.  Measured on MI355X (us graph-replayed, | issued one by
-// one; waves/splits; workgroups without splits x tiles of a sequence):
+// cannot fill the chip wants them on many waves.  Long launches end with their fullest CU (of 256): the
+// splits are those that spread the workgroups evenly.  Measured on MI355X (us graph-replayed, | issued one
+// by one; waves/splits; workgroups without splits x tiles of a sequence; head size 128, w: the wide form):
 //   512 x 112 (64 x 8192 tokens, 8 bit): 4/1 154, 4/2 156, 8/1 172; 512 x 32: 42 / 45 / 49; 512 x 13: 19 / 24 / 22
 //   512 x 33 (16 bit): 4/1 45, 4/2 49, 8/1 52; 512 x 64: 75 / 80 / 86; 2048 x 4: 22 / 41 / 43
-//   256 x 13: 4/1 12.5, 8/1 13.1, 4/2 15.0; 192 x 65 (head 64): 4/1 29, 4/2 22, 4/4 21, 8/1 21
-//   128 x 128: 4/1 58, 4/2 43, 4/4 43, 8/1 55; 32 x 512: 4/4 60, 4/8 43, 8/8 50
-//    64 x 65: 4/4 16.7, 4/8 15.7, 8/1 22; 64 x 49: 4/4 14.5, 4/8 15.9, 8/1 19; 64 x 25: 4/4 9.4, 8/1 9.4
+//   320 x 128 (16 bit): 4/1 113, 4/2 101; 320 x 64: 62 / 56; 320 x 32: 33 / 31; 320 x 13: 16 / 18; 400 x 64: 61 / 65
+//   256 x 13: 4/1 12.5, 8/1 13.1, 4/2 15.0; 224 x 65: 4/1 37, 4/2 40, w/1 41; 192 x 65: 34 / 37 / 37
+//   240 x 79 (head 64): 4/1 35, 4/2 29, w/1 31; 204 x 79 (head 64): 35 / 26 / 27; (head 32): 33 / 24 / 19
+//   136 x 65: 4/1 32, 4/2 33, 4/3 28, w/1 31; 136 x 129 (16 bit): 50 / 57 / 46 / 55
+//   192 x 33: w/1 18, 4/1 20; 160 x 33: w/1 16, 4/1 19, 4/3 19; 136 x 33: 15 / 19 / 18; 136 x 41 (16 bit): 16 / 19 / 19
+//    96 x 42 (16 bit): w/1 12.8, 4/2 14.6; 96 x 65 (16 bit): 23 / 19; 136 x 54 (16 bit, head 96): 17, 4/3 18
+//   128 x 128: 4/1 58, 4/2 43, 4/4 43, 8/1 55; 96 x 129 (16 bit): 4/2 33, 4/3 43, 4/5 33; 32 x 512: 4/4 60, 4/8 43, 8/8 50
+//    64 x 65: 4/4 16.7, 4/8 15.7, 8/1 22; 64 x 49: 4/4 14.5, 4/8 15.9, 8/1 19; 40 x 257 (16 bit): 4/6 28, 4/7 35
 //    64 x 13: 12/1 8.4 | 7.8, 4/4 8.7 | 8.5, 4/1 10; 32 x 13: 12/1 7.5 | 7.3, 4/4 8.4 | 8.4
 //    12 x 13 (head 64): 16/1 7.4 | 7.1, 4/4 6.7 | 8.4, 4/1 8.5; 8 x 7: 12/1 6.5 | 6.2, 4/2 7.5 | 8.4
 //     8 x 32: 12/3 8.6 | 8.5, 4/8 8.5 | 8.5, 12/1 11; 8 x 65: 8/9 8.2, 4/8 11; 6 x 24 (head 64): 16/1 7.7 | 7.4
@@ -57,14 +63,20 @@ static WinShape window_shape(int num_seqs, int num_heads, int num_kv_heads, int 
   const int64_t tiles = (seen + tok - 1) / tok + (window > 0 && seen < max_seq_len ? 1 + (sinks > 0) : 0);
   const int wide = win_wide(head_size, step);
   WinShape s{4, 1};
-  if (tiles <= 4 || wgs >= 256) return s;  // nothing to share out, or the chip is full
-  if (wgs * tiles <= 4352 && tiles <= 2 * wide) {  // one launch, at most two tiles per wave
+  if (tiles <= 4) return s;  // nothing to share out
+  if (wgs >= 256) {          // the chip is full; one and a half rounds instead of two
+    if (wgs > 256 && wgs <= 352 && tiles >= 32) s.splits = 2;
+  } else if (wgs * tiles <= 4352 && tiles <= 2 * wide) {  // one launch, at most two tiles per wave
     s.waves = wide;
   } else if (wgs * tiles <= 1024) {  // one tile per wave
     if (tiles > 32) s.waves = wide;
     s.splits = (int)((tiles + s.waves - 1) / s.waves);
-  } else {  // bound by bandwidth: a workgroup per CU
-    s.splits = (int)((256 + wgs - 1) / wgs);
+  } else if (wgs > 64 && tiles * head_size <= 56 * 128 && wgs * tiles * head_size <= 6000 * 128) {
+    s.waves = wide;  // splits would not fill the chip evenly, or cost more than they give
+  } else if (wgs <= 128) {  // bound by bandwidth: a workgroup per CU
+    s.splits = (int)(256 / wgs);
+  } else {  // three splits on every second CU; tiles of 8 KiB and less want the waves of two
+    s.splits = wgs <= 170 ? 3 : head_size <= 64 ? 2 : 1;
   }
   if (s.splits > WIN_MAX_SPLITS) s.splits = WIN_MAX_SPLITS;
   return s;
