@@ -354,3 +354,35 @@ def test_decode_step(ops, fmt, dtype, Hq, H, D, bs, window, sinks):
         ref, bound = plain.decode(q, kc, vc, sc, t, ln, window, sinks, D ** -0.5)
         plain.assert_within(out, ref, bound, f"step {step}")
     ops.check_device_diagnostics()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("S,Hq,H,D,longest", [
+    (9, 8, 8, 128, 3000),     # one workgroup of many waves per sequence and head, several tiles per wave
+    (34, 4, 4, 64, 8000),     # three splits
+    (17, 12, 12, 64, 8000),   # two splits of small tiles
+    (50, 6, 6, 32, 2500),     # two splits of more than 256 workgroups
+    (25, 8, 8, 96, 9000),     # none
+    (5, 8, 8, 80, 9000)])     # a workgroup per compute unit
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1200, 3)])
+def test_attention_and_step_launch_shapes(ops, fmt, S, Hq, H, D, longest, window, sinks):
+    """The launch is shaped by the longest sequence that may come; the ones that do are ragged, most of
+    them with nothing for most of the waves and splits."""
+    g = torch.Generator().manual_seed(S + D)
+    lens = [int(torch.randint(1, 60, (), generator=g)) for _ in range(S)]
+    lens[1], lens[S - 1], lens[2] = 1490, 777, 0
+    bs = 16
+    kc, vc, sc, t = filled(g, [n + 1 if n else 0 for n in lens], H, D, bs, fmt)
+    ln = torch.tensor(lens, dtype=torch.int32)
+    q = rows(g, S, Hq, D, torch.bfloat16)
+    out, _ = run_attention(ops, q, kc, vc, sc, t, ln, fmt, window, sinks, max_len=longest)
+    ref, bound = plain.decode(q, kc, vc, sc, t, ln, window, sinks, D ** -0.5)
+    plain.assert_within(out, ref, bound, "attention")
+    k, v = rows(g, S, H, D, torch.bfloat16, 3.0), rows(g, S, H, D, torch.bfloat16, 3.0)
+    ln = torch.where(ln > 0, ln + 1, ln)
+    out, dev = run_attention(ops, q, kc, vc, sc, t, ln, fmt, window, sinks, step=(k, v), max_len=longest)
+    plain.write(k, v, kc, vc, sc, t, ln, None, fmt)
+    assert all(same_bits(a, b) for a, b in zip(dev, (kc, vc, sc)))
+    ref, bound = plain.decode(q, kc, vc, sc, t, ln, window, sinks, D ** -0.5)
+    plain.assert_within(out, ref, bound, "step")
+    ops.check_device_diagnostics()

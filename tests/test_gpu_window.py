@@ -274,3 +274,30 @@ def test_decode_window_negative_scale_and_hidden_nan(ops):
         out = torch.empty_like(q).cuda()
         ops.paged_attention_window(out, q.cuda(), k2.cuda(), v2.cuda(), 2, scale, t.cuda(), ln.cuda(), 16, 90, 35, 3)
         plain.assert_within(out, ref, bound, f"scale {scale}")
+
+
+@pytest.mark.parametrize("S,Hq,H,D,longest", [
+    (9, 8, 8, 128, 1500),     # one workgroup of many waves per sequence and head, several tiles per wave
+    (34, 4, 4, 64, 5000),     # three splits
+    (17, 12, 12, 64, 5000),   # two splits of small tiles
+    (50, 12, 6, 32, 2500),    # two splits of more than 256 workgroups
+    (25, 8, 8, 96, 9000),     # none
+    (5, 8, 8, 80, 8000)])     # a workgroup per compute unit
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1200, 3)])
+def test_decode_window_launch_shapes(ops, S, Hq, H, D, longest, window, sinks):
+    """The launch is shaped by the longest sequence that may come; the ones that do are ragged, most of
+    them with nothing for most of the waves and splits."""
+    g = torch.Generator().manual_seed(S + D)
+    lens = [int(torch.randint(0, 60, (), generator=g)) for _ in range(S)]
+    lens[1], lens[S - 1], lens[2] = 1490, 777, 0
+    kc, vc, t = pool(g, lens, H, D, 16, torch.bfloat16)
+    ln = torch.tensor(lens, dtype=torch.int32)
+    q = rows(g, S, Hq, D, torch.bfloat16)
+    ref, bound = plain.decode(q, torch.nan_to_num(kc), torch.nan_to_num(vc, posinf=0.0), None, t, ln, window, sinks,
+                              D ** -0.5)
+    out = torch.full_like(q, float("nan")).cuda()
+    ops.paged_attention_window(out, q.cuda(), kc.cuda(), vc.cuda(), H, D ** -0.5, t.cuda(), ln.cuda(), 16, longest,
+                               window, sinks)
+    plain.assert_within(out, ref, bound, f"{S} x {H}, up to {longest}")
+    assert (out[2] == 0).all()
+    ops.check_device_diagnostics()
