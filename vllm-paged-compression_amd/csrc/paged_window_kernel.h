@@ -73,6 +73,18 @@ __device__ __forceinline__ float win_max_groups(float x) {
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 
+// max over the wave, in every lane: rotations inside the rows of 16 lanes, then row swaps
+__device__ __forceinline__ uint32_t win_max_wave(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x128, 0xf, 0xf, true));  // row_ror:8
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x124, 0xf, 0xf, true));  // row_ror:4
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x122, 0xf, 0xf, true));  // row_ror:2
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x121, 0xf, 0xf, true));  // row_ror:1
+  auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = max((uint32_t)a[0], (uint32_t)a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max((uint32_t)b[0], (uint32_t)b[1]);
+}
+
 // The tiles of a sequence that hold visible tokens: [0, sink_tiles) and [first, first + window
 // tiles); tokens are visible when tok < len and (tok >= lo or tok < sink_end).
 struct WinRange {
@@ -145,6 +157,13 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
   // the waves of all splits take the tiles in turn
   const int i0 = split * WAVES + wave, step = WAVES * a.num_splits;
   Ids ids = load_ids(a.window == 0 ? i0 : 0);
+  // STEP: the lane's two elements of the new row's key and of its value, requested in front of the tiles
+  uint32_t k_new = 0, v_new = 0;
+  if constexpr (STEP) {
+    const int e = min(lane, D / 2 - 1);
+    k_new = reinterpret_cast<const uint32_t*>((const T*)a.new_key + (int64_t)seq * a.new_k_stride + (int64_t)kvh * D)[e];
+    v_new = reinterpret_cast<const uint32_t*>((const T*)a.new_value + (int64_t)seq * a.new_v_stride + (int64_t)kvh * D)[e];
+  }
   const int raw_len = ((ConstInt)a.seq_lens)[seq];
   const int64_t most = (int64_t)a.table_width * BLK;
   const int len = raw_len > most ? (int)most : max(raw_len, 0);
@@ -433,6 +452,14 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
     }
   };
 
+  // dynamic LDS: o[WAVES][nh][16 * DT + 4], m[WAVES][16], l[WAVES][16] (f32), STEP: codes of the new row
+  extern __shared__ __attribute__((aligned(16))) float win_smem[];
+  constexpr int OROW = 16 * DT + 4;
+  const int heads = min(16, gqa);
+  float* sm_o = win_smem;
+  float* sm_m = win_smem + WAVES * heads * OROW;
+  float* sm_l = sm_m + WAVES * 16;
+
   // ---- STEP: the new row into the cache and the last tile ---------------------------------------
   // Returns whether the tile has to be read again: a row larger than everything before it changes the
   // older codes of its block, in memory (rare).
@@ -443,32 +470,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
       const int hn = (pos >> 4) - tile * NG, en = pos / ET - tile * NE;
       if (t.bad >> en & 1) return false;  // its block is outside the cache
       const int64_t blk = table[pos / BLK];
-      const T* krow = (const T*)a.new_key + (int64_t)seq * a.new_k_stride + (int64_t)kvh * D;
-      const T* vrow = (const T*)a.new_value + (int64_t)seq * a.new_v_stride + (int64_t)kvh * D;
-      u32x4 kx[KC][2];  // the lane's chunks of the key row: elements 16 * (4 kk + g) ..
-      uint16_t vx[DT];  // the lane's elements of the value row: 16 dt + c
-#pragma unroll
-      for (int kk = 0; kk < KC; ++kk) {
-        const int ch = min(4 * kk + g, CHUNKS - 1);
-        kx[kk][0] = *reinterpret_cast<const u32x4*>(krow + ch * 16);
-        kx[kk][1] = *reinterpret_cast<const u32x4*>(krow + ch * 16 + 8);
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) vx[dt] = reinterpret_cast<const uint16_t*>(vrow)[16 * dt + c];
-      uint32_t ka = 0, va = 0;
-#pragma unroll
-      for (int kk = 0; kk < KC; ++kk)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t w = kx[kk][e >> 2][e & 3];
-          ka = max(ka, max(finite_bits<T>(w & 0xffffu), finite_bits<T>(w >> 16)));
-        }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) va = max(va, finite_bits<T>(vx[dt]));
-#pragma unroll
-      for (int x = 16; x <= 32; x <<= 1) ka = max(ka, (uint32_t)__shfl_xor((int)ka, x));
-#pragma unroll
-      for (int x = 1; x <= 8; x <<= 1) va = max(va, (uint32_t)__shfl_xor((int)va, x));
+      const uint32_t ka = win_max_wave(max(finite_bits<T>(k_new & 0xffffu), finite_bits<T>(k_new >> 16)));
+      const uint32_t va = win_max_wave(max(finite_bits<T>(v_new & 0xffffu), finite_bits<T>(v_new >> 16)));
       auto old_scale = [&](int i) {
         return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.sc[i]), en * (64 / NE)));
       };
@@ -488,40 +491,43 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
           for (int it = lane; it < D * o; it += 64)
             reencode_byte<C>(reinterpret_cast<uint8_t*>(vw + it / o * BLK + it % o), vs_old * vi);
       }
+      // The lane's four codes, to memory as they are (V) and through LDS to the lanes whose registers they
+      // belong in: key codes in order, value codes (c, dt) at 8 c + dt.
+      const uint32_t codes = encode4<C>(bits_value<T>(k_new & 0xffffu) * ki, bits_value<T>(k_new >> 16) * ki,
+                                        bits_value<T>(v_new & 0xffffu) * vi, bits_value<T>(v_new >> 16) * vi);
+      uint8_t* row = reinterpret_cast<uint8_t*>(sm_l + WAVES * 16);
+      if (lane < D / 2) {
+        const int d = 2 * lane;
+        reinterpret_cast<uint16_t*>(row)[lane] = (uint16_t)codes;
+        row[128 + 8 * (d & 15) + (d >> 4)] = (uint8_t)(codes >> 16);
+        row[128 + 8 * ((d + 1) & 15) + (d >> 4)] = (uint8_t)(codes >> 24);
+        reinterpret_cast<uint8_t*>(vw)[d * BLK + o] = (uint8_t)(codes >> 16);
+        reinterpret_cast<uint8_t*>(vw)[(d + 1) * BLK + o] = (uint8_t)(codes >> 24);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (one wave: its LDS accesses stay in order)
+      __builtin_amdgcn_wave_barrier();
       // K: the row is token pos & 15 of group hn
+      const bool here = c == (pos & 15);
 #pragma unroll
-      for (int h = 0; h < NG; ++h) {
-        if (h != hn) continue;  // wave-uniform
-        const bool here = c == (pos & 15);
+      for (int kk = 0; kk < KC; ++kk) {
+        const int ch = min(4 * kk + g, CHUNKS - 1);
+        const u32x4 code = *reinterpret_cast<const u32x4*>(row + 16 * ch);
 #pragma unroll
-        for (int kk = 0; kk < KC; ++kk) {
-          u32x4 code;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const u32x4 x = kx[kk][w >> 1];
-            const uint32_t lo = x[(w & 1) * 2], hi = x[(w & 1) * 2 + 1];
-            code[w] = encode4<C>(bits_value<T>(lo & 0xffffu) * ki, bits_value<T>(lo >> 16) * ki,
-                                 bits_value<T>(hi & 0xffffu) * ki, bits_value<T>(hi >> 16) * ki);
-          }
-          if (here && 4 * kk + g < CHUNKS) {
-            t.k[h][kk] = code;
-            *reinterpret_cast<u32x4*>(kw + ((4 * kk + g) * BLK + o) * 16) = code;
-          }
-        }
+        for (int h = 0; h < NG; ++h)
+          if (here && h == hn) t.k[h][kk] = code;
+        if (here && 4 * kk + g < CHUNKS) *reinterpret_cast<u32x4*>(kw + (ch * BLK + o) * 16) = code;
       }
       // V: the lanes of group g hold its 16 tokens of row 16 dt + c; the row goes to byte pos & 15
       const bool mine = BLK == 32 ? (g >> 1) == (hn >> 1) : g == hn;
-      if (g == hn) {
-        const uint32_t sh = 8 * (pos & 3);
+      const u32x2 vc = *reinterpret_cast<const u32x2*>(row + 128 + 8 * c);
+      const uint32_t sh = 8 * (pos & 3);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t put = g == hn && ((pos & 15) >> 2) == w ? 0xffu << sh : 0u;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const uint32_t code = encode4<C>(bits_value<T>(vx[dt]) * vi, 0.f, 0.f, 0.f) & 255u;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t now = t.v[0][dt][w];
-            t.v[0][dt][w] = ((pos & 15) >> 2) == w ? (now & ~(0xffu << sh)) | (code << sh) : now;
-          }
-          reinterpret_cast<uint8_t*>(vw)[(16 * dt + c) * BLK + o] = (uint8_t)code;
+          const uint32_t code = (vc[dt >> 2] >> (8 * (dt & 3)) & 0xffu) << sh;
+          t.v[0][dt][w] = (t.v[0][dt][w] & ~put) | (code & put);
         }
       }
       const bool scaled = BLK == 8 ? lane * NE / 64 == en : mine;
@@ -562,13 +568,6 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
   }
-  // dynamic LDS: o[WAVES][nh][16 * DT + 4], m[WAVES][16], l[WAVES][16] (f32)
-  extern __shared__ __attribute__((aligned(16))) float win_smem[];
-  constexpr int OROW = 16 * DT + 4;
-  const int heads = min(16, gqa);
-  float* sm_o = win_smem;
-  float* sm_m = win_smem + WAVES * heads * OROW;
-  float* sm_l = sm_m + WAVES * 16;
   if (c < nh) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -637,7 +636,7 @@ template <typename T, typename C, int D, int WAVES, int BLK, bool STEP>
 inline void launch_window(const WinArgs& a, dim3 grid, hipStream_t st) {
   constexpr int DT = (D + 15) / 16;
   const int gqa = a.num_heads / a.num_kv_heads, heads = gqa < 16 ? gqa : 16;
-  const size_t lds = ((size_t)WAVES * heads * (16 * DT + 4) + 2 * WAVES * 16) * 4;
+  const size_t lds = ((size_t)WAVES * heads * (16 * DT + 4) + 2 * WAVES * 16) * 4 + (STEP ? 256 : 0);
   if (lds > 64 * 1024)
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_window_kernel<T, C, D, WAVES, BLK, STEP>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
