@@ -548,12 +548,15 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
   // only names table entries, which load_ids keeps inside the row.)
   for (int i = i0; i < R.tiles; i += step) {
     Tile t;
-    issue(t, at(i), ids);
-    if constexpr (STEP) {
-      if (i == early) {
-        if (raw_len > most) diag |= PE_DIAG_APPEND_MISMATCH;
-        else if (append(t, at(i))) issue(t, at(i), ids);
-      }
+    bool owner = STEP && i == early;
+    if (owner && raw_len > most) {
+      diag |= PE_DIAG_APPEND_MISMATCH;
+      owner = false;
+    }
+    while (true) {  // twice where the row grew its block's scale
+      issue(t, at(i), ids);
+      if (!owner || !append(t, at(i))) break;
+      owner = false;
     }
     ids = load_ids(at(i + step));
     compute(t, at(i));
