@@ -109,6 +109,8 @@ __host__ __device__ inline WinRange win_range(int len, int window, int sinks) {
 // does it.  Its block lies in the last tile, which one wave owns: that wave encodes the row, puts it
 // (and, where the block's scale grows, the re-expressed older codes) into the tile's registers and into
 // the cache, and goes on with the attention.  No other wave of the launch touches the block.
+// 64 x 776 tokens in e4m3: 20.6 us with the row, 18.6 without (the write in a launch of its own: 4.6);
+// 64 x 200: 11.3 and 8.6.  (Every lane encoding the chunks it holds: 21.8 and 13.6.)
 template <typename T, typename C, int D, int WAVES, int BLK, bool STEP>
 __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_window_kernel(const WinArgs a) {
   using TR = Traits<T>;
