@@ -386,3 +386,37 @@ def test_attention_and_step_launch_shapes(ops, fmt, S, Hq, H, D, longest, window
     ref, bound = plain.decode(q, kc, vc, sc, t, ln, window, sinks, D ** -0.5)
     plain.assert_within(out, ref, bound, "step")
     ops.check_device_diagnostics()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("bs", [8, 16, 32])
+def test_decode_step_special_rows(ops, fmt, bs):
+    """New rows of zeros, subnormals, infinities, NaN and the largest finite values, starting a block and
+    joining one: the codes and scales of the plain write; the outputs of the other sequences."""
+    g = torch.Generator().manual_seed(bs)
+    H, D = 2, 80
+    fills = [0.0, -0.0, 1e-40, 1e-30, 1e4, 3.3e38, float("inf"), float("-inf"), float("nan")]
+    S = 2 * len(fills)
+    lens = [2 * bs + 1] * len(fills) + [2 * bs + 4] * len(fills)
+    kc, vc, sc, t = filled(g, [n - 1 for n in lens], H, D, bs, fmt, spare=S + 5)
+    free = [b for b in range(vc.shape[0]) if b not in set(t.flatten().tolist())]
+    wide = torch.full((S, 3), -7, dtype=torch.int32)
+    wide[:, :t.shape[1]] = t
+    wide[:len(fills), 2] = torch.tensor(free[:len(fills)], dtype=torch.int32)
+    k, v = rows(g, S, H, D, torch.bfloat16), rows(g, S, H, D, torch.bfloat16)
+    for i, f in enumerate(fills + fills):
+        k[i, 0, ::7], v[i, 0, 3::5] = f, f
+        if i % 2:
+            k[i, 1], v[i, 1] = f, f
+    q = rows(g, S, 2 * H, D, torch.bfloat16)
+    ln = torch.tensor(lens, dtype=torch.int32)
+    out, dev = run_attention(ops, q, kc, vc, sc, wide, ln, fmt, 0, 0, step=(k, v))
+    plain.write(k, v, kc, vc, sc, wide, ln, None, fmt)
+    assert same_bits(dev[2], sc)
+    for got, want in zip(dev[:2], (kc, vc)):
+        got, want = got.cpu().float(), want.float()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    fine = [i for i in range(S) if abs((fills + fills)[i]) < 1e5]
+    ref, bound = plain.decode(q[fine], kc, vc, sc, wide[fine], ln[fine], 0, 0, D ** -0.5)
+    plain.assert_within(out[fine], ref, bound, "sequences with finite rows")
+    ops.check_device_diagnostics()
