@@ -1,0 +1,109 @@
+"""The 8-bit paged cache on the GPU where its rules meet their ends: blocks of scale 0 and of scales that are
+no powers of two, f16 weights beside value blocks of zeros, scores far from zero, waves that take many tiles."""
+import pytest
+import torch
+
+import plain_window as plain
+from test_gpu_8bit_cache import FORMATS, filled, garbage_cache, rows, run_attention, same_bits, tables_for
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import vllm_paged_compression_amd as pkg
+    import vllm_paged_compression_amd.ops as ops
+    pkg.load_library()
+    return ops
+
+
+def append(key, value, kc, vc, sc, t, lens, fmt):
+    """One row per sequence, from the definition, in place on CPU tensors: the block takes s = max(s_old, need), its
+    older codes become rn(code * s_old / s), also from s_old = 0; quotients are rounded to f32 first."""
+    bs = vc.shape[3]
+    for s, n in enumerate(lens.tolist()):
+        b, o = int(t[s, (n - 1) // bs]), (n - 1) % bs
+        for which, (new, cache, get) in enumerate(((key, kc, plain.k_rows), (value, vc, plain.v_rows))):
+            codes, block = get(cache, b), cache[b].clone()
+            for h in range(new.shape[1]):
+                x = new[s, h].double()
+                finite = x[torch.isfinite(x)].abs()
+                old = float(sc[b, h, which]) if o else 0.0
+                scale = max(old, plain.need_scale(float(finite.max()) if finite.numel() else 0.0, fmt))
+                if o and scale > old:
+                    plain.put(block, h, 0, plain.encode(codes[h, :o] * (old / scale), fmt), which)
+                quotient = (x / scale).float().double() if scale else x
+                plain.put(block, h, o, plain.encode(quotient, fmt)[None], which)
+                sc[b, h, which] = scale
+            cache[b] = block
+
+
+def same_values(a, b):
+    a, b = a.cpu().float(), b.float()
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+# ------------------------------------------------------------------ blocks whose scale is 0
+@pytest.mark.parametrize("how", ["write", "chunk", "step"])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,H,D,bs,older", [(4, 2, 64, 16, 1), (8, 1, 128, 8, 7), (2, 2, 80, 32, 19), (4, 2, 256, 16, 3),
+                                             (20, 1, 64, 16, 2)])
+def test_joining_a_block_of_zeros_and_infinities(ops, how, fmt, dtype, Hq, H, D, bs, older):
+    """Rows of zeros, infinities (the largest code) and NaN leave a block with scale 0: every element that is no NaN
+    reads as 0.  It still does after a finite row has given the block a scale."""
+    g = torch.Generator().manual_seed(older + D)
+    kc, vc, sc = garbage_cache(g, 9, H, D, bs, fmt)
+    lens = [older, bs + older]                       # the block is the sequence's first one, and its second
+    t = tables_for(g, 9, [3 * bs, 3 * bs], bs)
+    T = sum(lens)
+    k, v = rows(g, T, H, D, dtype), rows(g, T, H, D, dtype)
+    for x in (k, v):
+        for first in (0, T - older):
+            x[first:first + older] = 0
+            x[first, 0, 3], x[first + older - 1, H - 1, 7] = float("inf"), float("-inf")
+    v[0, 0, 5] = float("nan")
+    cu, ln = torch.tensor([0, lens[0], T], dtype=torch.int32), torch.tensor(lens, dtype=torch.int32)
+    dev = [x.cuda() for x in (kc, vc, sc)]
+    plain.write(k, v, kc, vc, sc, t, ln, cu, fmt)    # (these writes begin their blocks)
+    ops.reshape_and_cache_8bit(k.cuda(), v.cuda(), *dev, t.cuda(), ln.cuda(), cu.cuda(), max(lens), fmt)
+    assert float(dev[2][t[0, 0].long()].max()) == 0 and float(dev[2][t[1, 1].long()].max()) == 0
+    assert all(same_values(a, b) for a, b in zip(dev, (kc, vc, sc)))
+
+    for step in range(2):                            # the second one joins a block that has a scale
+        ln = ln + 1
+        k, v = (torch.ones(2, H, D, dtype=dtype) if step == 0 else rows(g, 2, H, D, dtype, 9.0) for _ in range(2))
+        k[1, 0, ::2], v[1, 0, ::2] = 0, 0
+        args = (k.cuda(), v.cuda(), *dev)
+        if how == "step":
+            q = rows(g, 2, Hq, D, dtype)
+            out = torch.empty_like(q).cuda()
+            ops.decode_step_8bit(out, q.cuda(), *args, H, D ** -0.5, t.cuda(), ln.cuda(), bs, 3 * bs, fmt)
+        else:
+            cu = torch.tensor([0, 1, 2], dtype=torch.int32).cuda() if how == "chunk" else None
+            ops.reshape_and_cache_8bit(*args, t.cuda(), ln.cuda(), cu, 1, fmt)
+        append(k, v, kc, vc, sc, t, ln, fmt)
+        assert same_bits(dev[2], sc), f"step {step}: scales"
+        for name, a, b in zip(("key codes", "value codes"), dev, (kc, vc)):
+            assert same_values(a, b), f"step {step}: {name}"
+        if how == "step":
+            # (the NaN of sequence 0 reaches its outputs)
+            ref, bound = plain.decode(q[1:], kc, vc, sc, t[1:], ln[1:], 0, 0, D ** -0.5)
+            plain.assert_within(out[1:], ref, bound, f"step {step}")
+    ops.check_device_diagnostics()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_joining_a_block_that_a_caller_gave_scale_zero(ops, fmt):
+    """Any codes under a scale of 0 (a cache made elsewhere) are zeros, whatever joins them."""
+    g = torch.Generator().manual_seed(5)
+    H, D, bs, S = 2, 64, 16, 3
+    kc, vc, sc, t = filled(g, [9, 3, 15], H, D, bs, fmt)
+    sc[t[:, 0].long()] = 0.0
+    ln = torch.tensor([10, 4, 16], dtype=torch.int32)
+    k, v, q = rows(g, S, H, D, torch.bfloat16), rows(g, S, H, D, torch.bfloat16), rows(g, S, 4, D, torch.bfloat16)
+    k[2], v[2] = 0, 0                               # nothing to scale: the codes stay as they are
+    out, dev = run_attention(ops, q, kc, vc, sc, t, ln, fmt, 0, 0, step=(k, v))
+    append(k, v, kc, vc, sc, t, ln, fmt)
+    assert all(same_bits(a, b) for a, b in zip(dev, (kc, vc, sc)))
+    plain.assert_within(out, *plain.decode(q, kc, vc, sc, t, ln, 0, 0, D ** -0.5))

@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64 * w8_waves(D, BLK)) void cache8_write_kernel(
       continue;
     }
     float* sc = kv_scales + ((int64_t)blk * num_kv_heads + h) * 2;
-    const float ks_old = o0 ? sc[0] : 0.f, vs_old = o0 ? sc[1] : 0.f;
+    const float ks_old = o0 ? sc[0] : 0.f, vs_old = o0 ? sc[1] : 0.f;  // (requested before the maxima)
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -106,24 +106,22 @@ __global__ __launch_bounds__(64 * w8_waves(D, BLK)) void cache8_write_kernel(
       ka = max(ka, red[0][w]);
       va = max(va, red[1][w]);
     }
-    const float ks = fmaxf(ks_old, pow2_scale<F>(bits_value<T>(ka)));
-    const float vs = fmaxf(vs_old, pow2_scale<F>(bits_value<T>(va)));
-    // exact for powers of two (a scale of 0 has no finite element but zeros to divide)
-    const float ki = ks > 0.f ? 1.f / ks : 1.f, vi = vs > 0.f ? 1.f / vs : 1.f;
+    const Joined kj = join_scale<F>(o0 > 0, ks_old, bits_value<T>(ka));
+    const Joined vj = join_scale<F>(o0 > 0, vs_old, bits_value<T>(va));
 
     uint8_t* kb = key_cache + blk * kv_block_stride + (int64_t)h * kv_head_stride;
     uint8_t* vb = value_cache + blk * kv_block_stride + (int64_t)h * kv_head_stride;
     // ---- older codes at the grown scale (rare: a row larger than everything before it) --------
-    if (ks_old > 0.f && ks > ks_old) {
+    if (kj.grew) {
       for (int it = tid; it < D / 16 * o0 * 4; it += THREADS)
-        reencode_word<F>(reinterpret_cast<uint32_t*>(kb + it / (o0 * 4) * (BLK * 16)) + it % (o0 * 4), ks_old * ki);
+        reencode_word<F>(reinterpret_cast<uint32_t*>(kb + it / (o0 * 4) * (BLK * 16)) + it % (o0 * 4), kj.factor());
     }
-    if (vs_old > 0.f && vs > vs_old) {
-      for (int it = tid; it < D * o0; it += THREADS) reencode_byte<F>(vb + it / o0 * BLK + it % o0, vs_old * vi);
+    if (vj.grew) {
+      for (int it = tid; it < D * o0; it += THREADS) reencode_byte<F>(vb + it / o0 * BLK + it % o0, vj.factor());
     }
     if (tid == 0) {
-      sc[0] = ks;
-      sc[1] = vs;
+      sc[0] = kj.scale;
+      sc[1] = vj.scale;
     }
     // ---- the new codes ------------------------------------------------------------------------
     const bool whole = o0 == 0 && o1 == BLK;
@@ -139,7 +137,7 @@ __global__ __launch_bounds__(64 * w8_waves(D, BLK)) void cache8_write_kernel(
         }
         return u32x2{encode4<F>(f[0], f[1], f[2], f[3]), encode4<F>(f[4], f[5], f[6], f[7])};
       };
-      const u32x2 kc = enc(kr[i], ki), vc = enc(vr[i], vi);
+      const u32x2 kc = enc(kr[i], kj.inv), vc = enc(vr[i], vj.inv);
       const int k_at = ((c >> 1) * BLK + slot) * 16 + (c & 1) * 8;
       if (whole) {
         // 8 elements x 4 tokens of a chunk, spread over the four lane groups -> two dwords per lane:

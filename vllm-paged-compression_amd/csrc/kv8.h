@@ -105,6 +105,26 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
+// The scale of a block that new rows join, 1 / scale, and what its older codes are multiplied by where the
+// scale grew.  `older`: the block has rows in front of the new ones; without them it begins anew, and what
+// memory holds as its scale does not count.  A scale of 0 stands for elements that all read as 0 (rows of
+// zeros and infinities leave non-zero codes under it): once it grows, the older codes become 0.
+struct Joined {
+  float old, scale, inv;
+  bool grew;
+  __device__ __forceinline__ float factor() const { return old * inv; }
+};
+template <typename F>
+__device__ __forceinline__ Joined join_scale(bool older, float stored, float amax) {
+  Joined j;
+  j.old = older ? stored : 0.f;
+  j.scale = fmaxf(j.old, pow2_scale<F>(amax));
+  // exact for powers of two (a scale of 0 has no finite element but zeros to divide)
+  j.inv = j.scale > 0.f ? 1.f / j.scale : 1.f;
+  j.grew = older && j.scale > j.old;
+  return j;
+}
+
 // magnitude bits of the finite elements of a packed pair of 16-bit values (0 for infinities and
 // NaN): they order like the magnitudes
 template <typename T>

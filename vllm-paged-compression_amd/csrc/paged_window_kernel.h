@@ -82,7 +82,7 @@ __device__ __forceinline__ uint32_t win_max_wave(uint32_t x) {
   auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   x = max((uint32_t)a[0], (uint32_t)a[1]);
   auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  return max((uint32_t)b[0], (uint32_t)b[1]);
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)max((uint32_t)b[0], (uint32_t)b[1]));
 }
 
 // The tiles of a sequence that hold visible tokens: [0, sink_tiles) and [first, first + window
@@ -477,26 +477,23 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
       auto old_scale = [&](int i) {
         return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.sc[i]), en * (64 / NE)));
       };
-      const float ks_old = o ? old_scale(0) : 0.f, vs_old = o ? old_scale(1) : 0.f;
-      const float ks = fmaxf(ks_old, pow2_scale<C>(bits_value<T>(ka)));
-      const float vs = fmaxf(vs_old, pow2_scale<C>(bits_value<T>(va)));
-      const float ki = ks > 0.f ? 1.f / ks : 1.f, vi = vs > 0.f ? 1.f / vs : 1.f;
+      const Joined kj = join_scale<C>(o > 0, old_scale(0), bits_value<T>(ka));
+      const Joined vj = join_scale<C>(o > 0, old_scale(1), bits_value<T>(va));
       char* kw = const_cast<char*>(kbase) + blk * blk_bytes;
       char* vw = const_cast<char*>(vbase) + blk * blk_bytes;
-      const bool k_grew = ks_old > 0.f && ks > ks_old, v_grew = vs_old > 0.f && vs > vs_old;
-      const bool grew = __builtin_amdgcn_ballot_w64(k_grew || v_grew) != 0;  // wave-uniform
+      const bool grew = __builtin_amdgcn_ballot_w64(kj.grew || vj.grew) != 0;  // wave-uniform
       if (grew) {
-        if (k_grew)
+        if (kj.grew)
           for (int it = lane; it < CHUNKS * o * 4; it += 64)
-            reencode_word<C>(reinterpret_cast<uint32_t*>(kw + it / (o * 4) * (BLK * 16)) + it % (o * 4), ks_old * ki);
-        if (v_grew)
+            reencode_word<C>(reinterpret_cast<uint32_t*>(kw + it / (o * 4) * (BLK * 16)) + it % (o * 4), kj.factor());
+        if (vj.grew)
           for (int it = lane; it < D * o; it += 64)
-            reencode_byte<C>(reinterpret_cast<uint8_t*>(vw + it / o * BLK + it % o), vs_old * vi);
+            reencode_byte<C>(reinterpret_cast<uint8_t*>(vw + it / o * BLK + it % o), vj.factor());
       }
       // The lane's four codes, to memory as they are (V) and through LDS to the lanes whose registers they
       // belong in: key codes in order, value codes (c, dt) at 8 c + dt.
-      const uint32_t codes = encode4<C>(bits_value<T>(k_new & 0xffffu) * ki, bits_value<T>(k_new >> 16) * ki,
-                                        bits_value<T>(v_new & 0xffffu) * vi, bits_value<T>(v_new >> 16) * vi);
+      const uint32_t codes = encode4<C>(bits_value<T>(k_new & 0xffffu) * kj.inv, bits_value<T>(k_new >> 16) * kj.inv,
+                                        bits_value<T>(v_new & 0xffffu) * vj.inv, bits_value<T>(v_new >> 16) * vj.inv);
       uint8_t* row = reinterpret_cast<uint8_t*>(sm_l + WAVES * 16);
       if (lane < D / 2) {
         const int d = 2 * lane;
@@ -533,10 +530,10 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
         }
       }
       const bool scaled = BLK == 8 ? lane * NE / 64 == en : mine;
-      if (scaled) t.sc = f32x2{ks, vs};
+      if (scaled) t.sc = f32x2{kj.scale, vj.scale};
       if (lane == 0) {
         float* sc = const_cast<float*>(a.kv_scales) + (blk * a.num_kv_heads + kvh) * 2;
-        *reinterpret_cast<f32x2*>(sc) = f32x2{ks, vs};
+        *reinterpret_cast<f32x2*>(sc) = f32x2{kj.scale, vj.scale};
       }
       if (grew) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "agent");  // the stores before the next loads
       return grew;
