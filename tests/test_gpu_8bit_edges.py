@@ -107,3 +107,36 @@ def test_joining_a_block_that_a_caller_gave_scale_zero(ops, fmt):
     append(k, v, kc, vc, sc, t, ln, fmt)
     assert all(same_bits(a, b) for a, b in zip(dev, (kc, vc, sc)))
     plain.assert_within(out, *plain.decode(q, kc, vc, sc, t, ln, 0, 0, D ** -0.5))
+
+
+# ------------------------------------------------------------------ f16 weights
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("gap", [5.0, 60.0, 80.0, 88.0, 90.0, 200.0, 3000.0])
+@pytest.mark.parametrize("where", ["same tile", "earlier tile", "later tile"])
+@pytest.mark.parametrize("bs", [8, 16, 32])
+def test_f16_peak_on_value_rows_of_zeros(ops, fmt, gap, where, bs):
+    """The heaviest keys lie in a block whose values are zeros (scale 0), `gap` nats above the rest.  A launch shaped
+    for one tile walks these nine tiles of 64 tokens with four waves: wave 0 takes tiles 0, 4 and 8."""
+    g = torch.Generator().manual_seed(bs)
+    H, D, n = 1, 64, 9 * 64
+    at = {"same tile": 4 * 64 + 32, "earlier tile": 0, "later tile": 8 * 64}[where]
+    kc, vc, sc = garbage_cache(g, n // bs + 2, H, D, bs, fmt)
+    t = tables_for(g, n // bs + 2, [n], bs)
+    k, v = 0.02 * rows(g, n, H, D, torch.float16), rows(g, n, H, D, torch.float16)
+    v[at:at + 32] = 0
+    q = torch.ones(1, 4, D, dtype=torch.float16)
+    k[at + 3] = gap * D ** 0.5 / D                    # q . k * scale = gap
+    cu, ln = torch.tensor([0, n], dtype=torch.int32), torch.tensor([n], dtype=torch.int32)
+    plain.write(k, v, kc, vc, sc, t, ln, cu, fmt)
+    ref, bound = plain.decode(q, kc, vc, sc, t, ln, 0, 0, D ** -0.5)
+    for max_len in (64, n):
+        out, _ = run_attention(ops, q, kc, vc, sc, t, ln, fmt, 0, 0, max_len=max_len)
+        plain.assert_within(out, ref, bound, f"launch shaped for {max_len} tokens")
+    new = torch.zeros(1, H, D, dtype=torch.float16)
+    # the step that starts a block with a row of zeros and a peak
+    wide = torch.cat([t, torch.tensor([[b for b in range(n // bs + 2) if b not in t[0].tolist()][:1]], dtype=torch.int32)], 1)
+    peak = new + k[at + 3]
+    out, dev = run_attention(ops, q, kc, vc, sc, wide, ln + 1, fmt, 0, 0, step=(peak, new), max_len=64)
+    append(peak, new, kc, vc, sc, wide, ln + 1, fmt)
+    assert all(same_bits(a, b) for a, b in zip(dev, (kc, vc, sc)))
+    plain.assert_within(out, *plain.decode(q, kc, vc, sc, wide, ln + 1, 0, 0, D ** -0.5), "step")

@@ -289,9 +289,10 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
   };
 
   float m_run = WIN_NEG, l_run = 0.f;  // log2 units; l_run: this lane's tokens only
-  float w_run = WIN_NEG;               // f16 with 8-bit values: reference point of p * scale
   // f16 products p * scale of V may leave f16's normal range; they are kept relative to their own
-  // running maximum.  bf16 has the range.
+  // running maximum 2^c_run (p being relative to 2^m_run).  bf16 has the range.  c_run follows differences
+  // of scores, which stay small where they matter however large the scores are.
+  float c_run = WIN_NEG;
   constexpr bool WREF = Q8 && __is_same(T, _Float16);
   f32x4 acc[DT];
 #pragma unroll
@@ -356,14 +357,18 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
       float y = -INFINITY, lv[NG];
 #pragma unroll
       for (int h = 0; h < NG; ++h) {
-        lv[h] = __builtin_amdgcn_logf(vs[h]);  // log2; -inf for a block of zeros
-        y = fmaxf(y, mx[h] + lv[h]);
+        // log2; -inf for a block of zeros and where nothing is visible (the scale may be anything)
+        lv[h] = mx[h] > -INFINITY ? __builtin_amdgcn_logf(vs[h]) : -INFINITY;
+        // A block of zeros moves the scores' maximum and not c: a group may lie any distance below the one and
+        // at the top of the other.  Counted as no lower than 2^-126 (where p becomes 0 anyway) it keeps its factor
+        // 2^(lv - c) within 2^126, so that 0 times the factor is 0.
+        y = fmaxf(y, fmaxf(mx[h] - m_new, -126.f) + lv[h]);
       }
-      const float w_new = fmaxf(w_run, win_max_groups(y));
-      alpha = __builtin_amdgcn_exp2f(w_run - w_new);
+      const float c_old = c_run + (m_run - m_new);
+      c_run = fmaxf(fmaxf(c_old, win_max_groups(y)), WIN_NEG);
+      alpha = __builtin_amdgcn_exp2f(c_old - c_run);
 #pragma unroll
-      for (int h = 0; h < NG; ++h) vs[h] = __builtin_amdgcn_exp2f(lv[h] + (m_new - w_new));
-      w_run = w_new;
+      for (int h = 0; h < NG; ++h) vs[h] = __builtin_amdgcn_exp2f(lv[h] - c_run);
     }
     m_run = m_new;
     float w[NG][4];
@@ -566,7 +571,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
   l_run += __shfl_xor(l_run, 16);
   l_run += __shfl_xor(l_run, 32);
   if constexpr (WREF) {  // numerators relative to the same point as the sum
-    const float f = __builtin_amdgcn_exp2f(w_run - m_run);
+    const float f = __builtin_amdgcn_exp2f(c_run);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
   }
