@@ -140,3 +140,65 @@ def test_f16_peak_on_value_rows_of_zeros(ops, fmt, gap, where, bs):
     append(peak, new, kc, vc, sc, wide, ln + 1, fmt)
     assert all(same_bits(a, b) for a, b in zip(dev, (kc, vc, sc)))
     plain.assert_within(out, *plain.decode(q, kc, vc, sc, wide, ln + 1, 0, 0, D ** -0.5), "step")
+
+
+# ------------------------------------------------------------------ many tiles per wave, launch shapes
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("order", ["falling", "rising", "both"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_tiles_per_wave(ops, fmt, order, dtype):
+    """45 tiles on four waves, scores and value scales that rise or fall by turns along the sequence: both reference
+    points of f16 weights move often, and in unlike directions."""
+    g = torch.Generator().manual_seed(14)
+    H, D, bs, n = 2, 64, 16, 45 * 64 - 11
+    kc, vc, sc = garbage_cache(g, n // bs + 4, H, D, bs, fmt)
+    t = tables_for(g, n // bs + 4, [n], bs)
+    k, v = rows(g, n, H, D, dtype, 0.3), rows(g, n, H, D, dtype)
+    x = torch.linspace(0, 1, n)
+    ramp = {"falling": 1 - x, "rising": x, "both": (2 * x - 1).abs()}[order]
+    k = (k.float() + (25 * ramp * D ** -0.5).view(n, 1, 1)).to(dtype)             # scores move by 25 nats
+    v = (v.float() * torch.exp2(8 * (0.5 - ramp) + 3 * torch.sin(40 * x)).view(n, 1, 1)).to(dtype)
+    q = torch.ones(1, 8, D, dtype=dtype) + 0.2 * rows(g, 1, 8, D, dtype)
+    cu, ln = torch.tensor([0, n], dtype=torch.int32), torch.tensor([n], dtype=torch.int32)
+    plain.write(k, v, kc, vc, sc, t, ln, cu, fmt)
+    for window, sinks in ((0, 0), (2000, 100)):
+        ref, bound = plain.decode(q, kc, vc, sc, t, ln, window, sinks, D ** -0.5)
+        for max_len in (64, n, 1 << 20):
+            out, _ = run_attention(ops, q, kc, vc, sc, t, ln, fmt, window, sinks, max_len=max_len)
+            plain.assert_within(out, ref, bound, f"window {window}, launch shaped for {max_len} tokens")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("S,Hq,H,D,longest", [(9, 8, 8, 128, 3000), (34, 4, 4, 64, 8000), (17, 12, 12, 64, 8000),
+                                              (50, 6, 6, 32, 2500), (25, 8, 8, 96, 9000), (5, 8, 8, 80, 9000)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1200, 3)])
+def test_f16_launch_shapes(ops, fmt, S, Hq, H, D, longest, window, sinks):
+    """The launch shapes with f16 rows: partials whose weights have their own reference points, joined."""
+    g = torch.Generator().manual_seed(S + D)
+    lens = [int(torch.randint(1, 60, (), generator=g)) for _ in range(S)]
+    lens[1], lens[S - 1], lens[2] = 1490, 777, 0
+    bs, dtype = 16, torch.float16
+    kc, vc, sc, t = filled(g, [n + 1 if n else 0 for n in lens], H, D, bs, fmt, dtype)
+    ln = torch.tensor(lens, dtype=torch.int32)
+    q = rows(g, S, Hq, D, dtype)
+    out, _ = run_attention(ops, q, kc, vc, sc, t, ln, fmt, window, sinks, max_len=longest)
+    plain.assert_within(out, *plain.decode(q, kc, vc, sc, t, ln, window, sinks, D ** -0.5), "attention")
+    k, v = rows(g, S, H, D, dtype, 3.0), rows(g, S, H, D, dtype, 3.0)
+    ln = torch.where(ln > 0, ln + 1, ln)
+    out, dev = run_attention(ops, q, kc, vc, sc, t, ln, fmt, window, sinks, step=(k, v), max_len=longest)
+    plain.write(k, v, kc, vc, sc, t, ln, None, fmt)
+    assert all(same_bits(a, b) for a, b in zip(dev, (kc, vc, sc)))
+    plain.assert_within(out, *plain.decode(q, kc, vc, sc, t, ln, window, sinks, D ** -0.5), "step")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [1024 * 64 - 5, 1024 * 64 + 70])
+def test_one_long_request_on_one_kv_head(ops, dtype, n):
+    """Both sides of 1024 tiles of one (sequence, KV head), where the launch changes its shape."""
+    g = torch.Generator().manual_seed(15)
+    D, bs = 32, 32
+    kc, vc, sc, t = filled(g, [n], 1, D, bs, "int8", dtype)
+    ln = torch.tensor([n], dtype=torch.int32)
+    q = rows(g, 1, 4, D, dtype)
+    out, _ = run_attention(ops, q, kc, vc, sc, t, ln, "int8", 0, 0)
+    plain.assert_within(out, *plain.decode(q, kc, vc, sc, t, ln, 0, 0, D ** -0.5))
