@@ -694,9 +694,10 @@ typedef enum { PE_KV_SAME = 0, PE_KV_FP8_E4M3 = 1, PE_KV_INT8 = 2 } pe_kv_format
  *           a block begins anew there, whatever it held
  *   codes   rn(x / s), to nearest even; where s grew, the block's older codes become
  *           rn(code * s_old / s)
- * x / s is exact (powers of two).  The scale is taken from finite elements; infinities become the
- * largest code, NaN stays NaN (e4m3) or becomes 0 (int8).  Slots behind a sequence's last row are
- * left as they are.  Two sequences must not append to one block. */
+ * x / s is exact (powers of two), unless the block came with another scale from elsewhere (any finite
+ * f32 >= 0): then the quotient, or code * s_old / s, is rounded to f32 first.  The scale is taken from
+ * finite elements; infinities become the largest code, NaN stays NaN (e4m3) or becomes 0 (int8).  Slots
+ * behind a sequence's last row are left as they are.  Two sequences must not append to one block. */
 int pe_reshape_and_cache_8bit(const void* key, const void* value, void* key_cache, void* value_cache,
                               float* kv_scales, const int32_t* block_tables, const int32_t* seq_lens,
                               const int32_t* cu_q, int num_seqs, int64_t num_tokens, int max_q_len,

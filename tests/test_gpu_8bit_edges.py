@@ -109,6 +109,43 @@ def test_joining_a_block_that_a_caller_gave_scale_zero(ops, fmt):
     plain.assert_within(out, *plain.decode(q, kc, vc, sc, t, ln, 0, 0, D ** -0.5))
 
 
+# ------------------------------------------------------------------ blocks whose scale is no power of two
+@pytest.mark.parametrize("how", ["write", "step"])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_joining_blocks_of_any_scale(ops, how, fmt, dtype):
+    """Scales of a cache made elsewhere: x / s is rounded once to f32 (x times a rounded 1 / s falls off the ties of
+    these rows), also where 1 / s is past f32's largest number."""
+    g = torch.Generator().manual_seed(6)
+    H, D, bs, S = 2, 64, 16, 60
+    # x / s lies on the tie `half` in f32, x * (1 / s) next to it
+    x = torch.arange(128.0, 256.0)[:, None]
+    half = torch.arange(8) + 0.5 if fmt == "int8" else torch.arange(17.0, 32.0, 2)[:8]
+    scale = x / half
+    apart = (x / scale == half) & (x * (1 / scale) != half)
+    at = apart.nonzero()
+    at = at[torch.randperm(len(at), generator=g)[:S - 3]]
+    assert len(at) == S - 3
+    kc, vc, sc, t = filled(g, [5] * S, H, D, bs, fmt)
+    k, v = torch.zeros(S, H, D, dtype=dtype), torch.zeros(S, H, D, dtype=dtype)
+    for s, (i, j) in enumerate(at.tolist()):
+        sc[t[s, 0].long()] = scale[i, j]
+        k[s], v[s, :, 3:] = float(x[i]), -float(x[i])
+    for s, tiny in zip(range(S - 3, S), (1e-39, 2.0 ** -149, 2.0 ** -130)):
+        sc[t[s, 0].long()] = tiny                        # rows of zeros leave it
+    sc[t[0, 0].long(), :, 0], k[0] = 0.0, 0              # nothing to divide beside a quotient
+    ln = torch.full((S,), 6, dtype=torch.int32)
+    if how == "step":
+        q = rows(g, S, 4, D, dtype)
+        _, dev = run_attention(ops, q, kc, vc, sc, t, ln, fmt, 0, 0, step=(k, v))
+    else:
+        dev = [x.cuda() for x in (kc, vc, sc)]
+        ops.reshape_and_cache_8bit(k.cuda(), v.cuda(), *dev, t.cuda(), ln.cuda(), None, 1, fmt)
+    append(k, v, kc, vc, sc, t, ln, fmt)
+    for name, a, b in zip(("key codes", "value codes", "scales"), dev, (kc, vc, sc)):
+        assert same_bits(a, b), name
+
+
 # ------------------------------------------------------------------ f16 weights
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("gap", [5.0, 60.0, 80.0, 88.0, 90.0, 200.0, 3000.0])

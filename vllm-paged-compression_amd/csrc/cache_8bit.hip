@@ -4,8 +4,8 @@
 //   need = 2^ceil(log2(max |x| / FMAX)) over the block's new (finite) elements,
 //   s    = max(s_old, need),  s_old = 0 when the call writes the block's offset 0,
 //   code = rn(x / s);  older codes of a block whose s grew:  code <- rn(code * s_old / s).
-// With powers of two x / s is exact and a code is rounded once; re-expressing e4m3 codes only
-// rounds those that become subnormal.
+// With powers of two x / s is exact and a code is rounded once (under a caller's scale, which may be any
+// number, x / s is rounded to f32 first); re-expressing e4m3 codes only rounds those that become subnormal.
 //
 // One workgroup owns one (sequence, block, KV head): the maximum over the block's new rows, the
 // re-expression of its older codes and the scale are decided in one place, without atomics.  A wave
@@ -16,6 +16,8 @@
 // Bound: HBM (2 bytes read, 1 written per element): 4 x 8192 rows of 8 x 128, int8, 39 us (4.7 TB/s, a
 // copy's rate); a decode step (one row per sequence) by the chain of dependent loads lengths -> rows /
 // table -> scale: 64 x 8 x 128, 4.6 us.
+#include <type_traits>
+
 #include "kv8.h"
 
 namespace pe {
@@ -128,16 +130,17 @@ __global__ __launch_bounds__(64 * w8_waves(D, BLK)) void cache8_write_kernel(
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const int item = wave * I + i, slot = item / CG * 4 + g, c = item % CG * 16 + c16;
-      auto enc = [&](const u32x4& r, float inv) {
+      auto enc = [&](const u32x4& r, const Joined& j, auto exact) {
+        constexpr bool EXACT = decltype(exact)::value;
         float f[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          f[2 * e] = bits_value<T>(r[e] & 0xffffu) * inv;
-          f[2 * e + 1] = bits_value<T>(r[e] >> 16) * inv;
+          f[2 * e] = j.divide<EXACT>(bits_value<T>(r[e] & 0xffffu));
+          f[2 * e + 1] = j.divide<EXACT>(bits_value<T>(r[e] >> 16));
         }
         return u32x2{encode4<F>(f[0], f[1], f[2], f[3]), encode4<F>(f[4], f[5], f[6], f[7])};
       };
-      const u32x2 kc = enc(kr[i], kj.inv), vc = enc(vr[i], vj.inv);
+      u32x2 kc = enc(kr[i], kj, std::true_type{}), vc = enc(vr[i], vj, std::true_type{});
       const int k_at = ((c >> 1) * BLK + slot) * 16 + (c & 1) * 8;
       if (whole) {
         // 8 elements x 4 tokens of a chunk, spread over the four lane groups -> two dwords per lane:
@@ -154,6 +157,8 @@ __global__ __launch_bounds__(64 * w8_waves(D, BLK)) void cache8_write_kernel(
           v[BLK / 4] = d1;
         }
       } else if (slot >= o0 && slot < o1 && c < CH) {
+        if (!kj.exact) kc = enc(kr[i], kj, std::false_type{});  // (only a block with older rows has a scale from elsewhere)
+        if (!vj.exact) vc = enc(vr[i], vj, std::false_type{});
         *reinterpret_cast<u32x2*>(kb + k_at) = kc;
 #pragma unroll
         for (int e = 0; e < 8; ++e) vb[(c * 8 + e) * BLK + slot] = (uint8_t)(vc[e >> 2] >> (8 * (e & 3)));

@@ -109,18 +109,27 @@ __device__ __forceinline__ float pow2_scale(float amax) {
 // scale grew.  `older`: the block has rows in front of the new ones; without them it begins anew, and what
 // memory holds as its scale does not count.  A scale of 0 stands for elements that all read as 0 (rows of
 // zeros and infinities leave non-zero codes under it): once it grows, the older codes become 0.
+// All arguments are the same in every lane of the wave.
 struct Joined {
   float old, scale, inv;
-  bool grew;
+  bool grew, exact;
   __device__ __forceinline__ float factor() const { return old * inv; }
+  // x / scale, rounded once to f32.  Scales that a write chose are powers of two (and a scale of 0 has no finite
+  // element but zeros to divide): x times 1 / scale is the quotient itself.  A cache made elsewhere may hold any
+  // scale, also one whose 1 / scale is rounded or past f32's largest number.
+  // (EXACT: the caller has looked)
+  template <bool EXACT>
+  __device__ __forceinline__ float divide(float x) const {
+    return EXACT || exact ? x * inv : x / scale;
+  }
 };
 template <typename F>
 __device__ __forceinline__ Joined join_scale(bool older, float stored, float amax) {
   Joined j;
   j.old = older ? stored : 0.f;
   j.scale = fmaxf(j.old, pow2_scale<F>(amax));
-  // exact for powers of two (a scale of 0 has no finite element but zeros to divide)
   j.inv = j.scale > 0.f ? 1.f / j.scale : 1.f;
+  j.exact = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(j.scale) & 0x7fffffu)) == 0;  // 0, or 2^k >= 2^-126
   j.grew = older && j.scale > j.old;
   return j;
 }

@@ -497,8 +497,12 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
       }
       // The lane's four codes, to memory as they are (V) and through LDS to the lanes whose registers they
       // belong in: key codes in order, value codes (c, dt) at 8 c + dt.
-      const uint32_t codes = encode4<C>(bits_value<T>(k_new & 0xffffu) * kj.inv, bits_value<T>(k_new >> 16) * kj.inv,
-                                        bits_value<T>(v_new & 0xffffu) * vj.inv, bits_value<T>(v_new >> 16) * vj.inv);
+      auto enc = [&](auto exact) {
+        constexpr bool EXACT = decltype(exact)::value;
+        return encode4<C>(kj.divide<EXACT>(bits_value<T>(k_new & 0xffffu)), kj.divide<EXACT>(bits_value<T>(k_new >> 16)),
+                          vj.divide<EXACT>(bits_value<T>(v_new & 0xffffu)), vj.divide<EXACT>(bits_value<T>(v_new >> 16)));
+      };
+      const uint32_t codes = kj.exact && vj.exact ? enc(std::true_type{}) : enc(std::false_type{});
       uint8_t* row = reinterpret_cast<uint8_t*>(sm_l + WAVES * 16);
       if (lane < D / 2) {
         const int d = 2 * lane;
