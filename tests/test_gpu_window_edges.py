@@ -1,0 +1,46 @@
+"""Windowed attention on the GPU at the ends of its inputs: no kv rows, no requests, grids past a dimension's
+limit, scores far from zero."""
+import pytest
+import torch
+
+import plain_window as plain
+from test_gpu_window import pool, prefill_reference, rows, run_prefill
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import vllm_paged_compression_amd as pkg
+    import vllm_paged_compression_amd.ops as ops
+    pkg.load_library()
+    return ops
+
+
+def cu(*sums):
+    return torch.tensor(sums, dtype=torch.int32).cuda()
+
+
+# ------------------------------------------------------------------ no kv rows
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 0), (20, 3)])
+def test_prefill_without_kv_rows(ops, D, window, sinks):
+    """No request has a kv row: zeros for their queries, the rows behind the last request left as they were."""
+    g = torch.Generator().manual_seed(1)
+    q = rows(g, 80, 4, D, torch.bfloat16).cuda()
+    none = torch.empty(0, 2, D, dtype=torch.bfloat16, device="cuda")
+    out = torch.full((80, 4, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = ops.prefill_window(q, none, none, cu(0, 1, 70), cu(0, 0, 0), 69, 0.1, window, sinks, out)
+    assert got is out and (out[:70] == 0).all()
+    assert (out[70:] == 7).all(), "rows behind the last request were touched"
+    # (prefix sums that name rows which are not there are cut)
+    out.fill_(7)
+    ops.prefill_window(q, none, none, cu(0, 1, 70), cu(0, 5, 300), 69, 0.1, window, sinks, out)
+    assert (out[:70] == 0).all() and (out[70:] == 7).all()
+
+
+def test_prefill_without_kv_rows_refuses_what_the_call_refuses(ops):
+    q = torch.zeros(3, 4, 72, dtype=torch.bfloat16, device="cuda")
+    none = torch.empty(0, 2, 72, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="head size"):
+        ops.prefill_window(q, none, none, cu(0, 3), cu(0, 0), 3, 0.1, 5)

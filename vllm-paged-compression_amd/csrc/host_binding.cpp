@@ -341,9 +341,7 @@ PyObject* prefill_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const int dev = device_of({&q, &k, &v, &cu_q, &cu_kv, out.defined() ? &out : nullptr});
     if (!out.defined()) out = at::empty({q.size(0), Hq, D}, q.options());
-    if (k.size(0) == 0) {  // nothing to attend
-      out.zero_();
-    } else if (q.size(0) > 0 && cu_q.size(0) > 1) {
+    if (q.size(0) > 0 && cu_q.size(0) > 1) {  // (without kv rows too: the kernel writes the zeros of the requests' rows)
       launch(what, dev, [&](void* st) {
         return pe_prefill_window(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                  (const int32_t*)cu_q.data_ptr(), (const int32_t*)cu_kv.data_ptr(),

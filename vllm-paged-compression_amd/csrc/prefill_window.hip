@@ -15,7 +15,9 @@ extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const 
   PE_REQUIRE(sliding_window >= 0 && num_sinks >= 0, PE_ERR_INVALID_ARG,
              "prefill_window: sliding_window %d and num_sinks %d must not be negative", sliding_window, num_sinks);
   if (num_seqs == 0 || max_q_len == 0 || num_q_rows == 0) return PE_OK;
-  PE_REQUIRE(out && q && k && v && cu_q && cu_kv, PE_ERR_INVALID_ARG, "prefill_window: null pointer");
+  // (without kv rows k and v are not read, and an empty tensor has no address)
+  PE_REQUIRE(out && q && (num_kv_rows == 0 || (k && v)) && cu_q && cu_kv, PE_ERR_INVALID_ARG,
+             "prefill_window: null pointer");
   PE_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0, PE_ERR_INVALID_ARG,
              "prefill_window: num_heads %d must be a positive multiple of num_kv_heads %d", num_heads, num_kv_heads);
   PE_REQUIRE(head_size == 32 || head_size == 64 || head_size == 80 || head_size == 96 || head_size == 112 ||
