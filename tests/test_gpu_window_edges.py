@@ -44,3 +44,19 @@ def test_prefill_without_kv_rows_refuses_what_the_call_refuses(ops):
     none = torch.empty(0, 2, 72, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError, match="head size"):
         ops.prefill_window(q, none, none, cu(0, 3), cu(0, 0), 3, 0.1, 5)
+
+
+# ------------------------------------------------------------------ nothing to launch
+@pytest.mark.parametrize("what", ["no requests", "max_q_len 0"])
+def test_prefill_that_launches_nothing_returns_zeros(ops, what):
+    """A fresh output is not left with what its memory held."""
+    q, k = (torch.ones(50, h, 64, dtype=torch.float16, device="cuda") for h in (4, 2))
+    for _ in range(4):
+        dirty = torch.full((50, 4, 64), float("nan"), dtype=torch.float16, device="cuda")
+        del dirty                                      # the allocator hands the same memory out again
+        sums = cu(0) if what == "no requests" else cu(0, 0)
+        got = ops.prefill_window(q, k, k, sums, sums, 0, 0.1, 5)
+        assert got.shape == q.shape and (got == 0).all()
+    out = torch.full((50, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    ops.prefill_window(q, k, k, sums, sums, 0, 0.1, 5, 0, out)
+    assert (out == 7).all()                            # a caller's output keeps the rows of no request

@@ -1054,8 +1054,10 @@ def prefill_window(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
                    num_sinks: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``prefill_causal`` through a window: query i of a request attends its kv rows j <=
     min(i, Lkv-1) with j > i - ``sliding_window`` (0: all of them) or j < ``num_sinks``; a query that
-    sees none gets zeros.  query [Tq, Hq, D], key/value [Tkv, Hkv, D] bf16 or f16; cu_q/cu_kv int32
-    prefix sums; ``max_q_len`` = the longest request."""
+    sees none gets zeros.  query [Tq, Hq, D], key/value [Tkv, Hkv, D] bf16 or f16 (f32 is refused);
+    ``scale`` > 0; cu_q/cu_kv int32 prefix sums; ``max_q_len`` = the longest request.  Rows of ``out`` that
+    belong to no request, or lie past ``max_q_len`` in theirs, are not written; a fresh output holds
+    zeros if there is no request or ``max_q_len`` is 0, and anything in such rows otherwise."""
     return (_lib._host or _lib.load_host()).prefill_window(
         query, key, value, cu_q, cu_kv, max_q_len, scale, sliding_window, num_sinks, out)
 
