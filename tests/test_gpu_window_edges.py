@@ -60,3 +60,16 @@ def test_prefill_that_launches_nothing_returns_zeros(ops, what):
     out = torch.full((50, 4, 64), 7.0, dtype=torch.float16, device="cuda")
     ops.prefill_window(q, k, k, sums, sums, 0, 0.1, 5, 0, out)
     assert (out == 7).all()                            # a caller's output keeps the rows of no request
+
+
+# ------------------------------------------------------------------ grids
+@pytest.mark.parametrize("Hq,H,D", [(4, 1, 64), (4, 1, 128), (8, 1, 256)])
+@pytest.mark.parametrize("max_q_len", [16 * 65535, 16 * 65535 + 1, 64 * 65535])
+def test_prefill_max_q_len_far_above_the_prompts(ops, Hq, H, D, max_q_len):
+    """max_q_len sizes the grid: with the query heads of a KV head side by side a workgroup takes 16 rows, which
+    more than 65535 workgroups in a row would have to cover."""
+    g = torch.Generator().manual_seed(2)
+    lens = [100, 31]
+    q, k, v = (rows(g, 131, h, D, torch.bfloat16) for h in (Hq, H, H))
+    got = ops.prefill_window(q.cuda(), k.cuda(), v.cuda(), cu(0, 100, 131), cu(0, 100, 131), max_q_len, D ** -0.5, 17, 2)
+    plain.assert_within(got, *prefill_reference(q, k, v, lens, lens, 17, 2, D ** -0.5))

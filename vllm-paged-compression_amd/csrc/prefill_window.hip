@@ -40,7 +40,8 @@ extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const 
   hipStream_t st = static_cast<hipStream_t>(stream);
   const float sl2 = scale * 1.4426950408889634f;
   // Tile shape: 16 x NR query rows per wave, 4 waves (8 at the 256 pitch), BN keys per tile; the waves
-  // take the query heads of a KV head side by side (hpw of them).  Measured on MI355X (us per launch over
+  // take the query heads of a KV head side by side (hpw of them; fewer where the blocks of 16 * NR * waves / hpw
+  // rows would be more than the 65535 of a grid dimension).  Measured on MI355X (us per launch over
   // three sets of inputs; NR x BN = 2 x 64 / 1 x 64 / 1 x 32; 32 query and 8 KV heads x 128, 4 sinks; none
   // = no window):
   //   8 x 1024 tokens, window 64: 59 / 71 / 48, 128: 64 / 75 / 57, 256: 73 / 88 / 74, 384: 79 / 98 / 83,
@@ -57,9 +58,10 @@ extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const 
 #define PE_LAUNCH_PW(T, HS, NR, WAVES, WPE, BN)                                                         \
   do {                                                                                                  \
     int hpw = WAVES;                                                                                    \
-    while (gqa % hpw) hpw /= 2;                                                                         \
-    const int bm = 16 * NR * WAVES / hpw;                                                               \
-    dim3 grid((unsigned)(num_heads / hpw), (unsigned)num_seqs, (unsigned)((max_q_len + bm - 1) / bm));  \
+    auto row_blocks = [&] { return (max_q_len + 16 * NR * WAVES / hpw - 1) / (16 * NR * WAVES / hpw); }; \
+    while (gqa % hpw || (hpw > 1 && row_blocks() > 65535)) hpw /= 2;                                    \
+    PE_REQUIRE(row_blocks() <= 65535, PE_ERR_UNSUPPORTED, "prefill_window: grid too large");             \
+    dim3 grid((unsigned)(num_heads / hpw), (unsigned)num_seqs, (unsigned)row_blocks());                 \
     const size_t lds = 4 * (size_t)BN * HS * 2;                                                         \
     if (lds > 64 * 1024)                                                                                \
       (void)hipFuncSetAttribute(                                                                        \
