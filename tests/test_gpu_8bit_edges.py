@@ -239,3 +239,28 @@ def test_one_long_request_on_one_kv_head(ops, dtype, n):
     q = rows(g, 1, 4, D, dtype)
     out, _ = run_attention(ops, q, kc, vc, sc, t, ln, "int8", 0, 0)
     plain.assert_within(out, *plain.decode(q, kc, vc, sc, t, ln, 0, 0, D ** -0.5))
+
+
+# ------------------------------------------------------------------ scores far from zero
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [1e4, 1e8, 1e9, 1e10, 1e25, 1e33])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_scores_far_from_zero(ops, fmt, dtype, size, sign):
+    """All scores near `sign * size`, one key ahead of the others by more than f32's step there: the output is the
+    value of that key, however far the scores are from zero."""
+    g = torch.Generator().manual_seed(16)
+    H, D, bs, n, ahead = 1, 64, 16, 200, 77
+    kc, vc, sc = garbage_cache(g, 16, H, D, bs, fmt)
+    t = tables_for(g, 16, [n], bs)
+    k, v = torch.full((n, H, D), 1.0, dtype=dtype), rows(g, n, H, D, dtype)
+    k[ahead] = 1.5 if sign > 0 else 0.5
+    cu, ln = torch.tensor([0, n], dtype=torch.int32), torch.tensor([n], dtype=torch.int32)
+    plain.write(k, v, kc, vc, sc, t, ln, cu, fmt)
+    sc[t[0].long(), :, 0] *= size / 8                  # K's scales carry the size
+    q = torch.full((1, 2, D), sign, dtype=dtype)
+    block, slot = int(t[0, ahead // bs]), ahead % bs
+    want = (plain.v_rows(vc, block)[0, slot] * float(sc[block, 0, 1])).to(dtype)
+    for max_len in (64, n, 1 << 16):
+        out, _ = run_attention(ops, q, kc, vc, sc, t, ln, fmt, 0, 0, max_len=max_len)
+        assert torch.equal(out.cpu(), want.expand(1, 2, D)), f"launch shaped for {max_len} tokens"

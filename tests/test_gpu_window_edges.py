@@ -73,3 +73,34 @@ def test_prefill_max_q_len_far_above_the_prompts(ops, Hq, H, D, max_q_len):
     q, k, v = (rows(g, 131, h, D, torch.bfloat16) for h in (Hq, H, H))
     got = ops.prefill_window(q.cuda(), k.cuda(), v.cuda(), cu(0, 100, 131), cu(0, 100, 131), max_q_len, D ** -0.5, 17, 2)
     plain.assert_within(got, *prefill_reference(q, k, v, lens, lens, 17, 2, D ** -0.5))
+
+
+# ------------------------------------------------------------------ scores far from zero
+def far_scores(dtype, D, size, sign, n, ahead):
+    """q, k with every score sign * size but one key's, which is ahead by half of it; D ** -0.5 scales."""
+    per = (size / D ** 0.5) ** 0.5
+    q = torch.full((n, 2, D), sign * per).to(dtype)
+    k = torch.full((n, 1, D), per).to(dtype)
+    k[ahead] *= 1.5 if sign > 0 else 0.5
+    return q, k
+
+
+SIZES = [(torch.float16, s) for s in (1e4, 1e8, 1e9, 1e10)] + [(torch.bfloat16, s) for s in (1e4, 1e9, 1e10, 1e25, 1e33)]
+
+
+@pytest.mark.parametrize("dtype,size", SIZES)
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_decode_window_scores_far_from_zero(ops, dtype, size, sign):
+    g = torch.Generator().manual_seed(4)
+    D, bs, n, ahead = 64, 16, 200, 77
+    kc, vc, t = pool(g, [n], 1, D, bs, dtype)
+    q, k = far_scores(dtype, D, size, sign, n, ahead)
+    for j in range(n):
+        kc[t[0, j // bs].long(), :, :, j % bs] = k[j].view(1, D // 8, 8)
+    want = vc[t[0, ahead // bs].long(), 0, :, ahead % bs]
+    ln = torch.tensor([n], dtype=torch.int32)
+    for max_len in (64, n, 1 << 16):
+        out = torch.empty_like(q[:1]).cuda()
+        ops.paged_attention_window(out, q[:1].cuda(), kc.cuda(), vc.cuda(), 1, D ** -0.5, t.cuda(), ln.cuda(), bs,
+                                   max_len, 150, 2)
+        assert torch.equal(out.cpu(), want.expand(1, 2, D)), f"launch shaped for {max_len} tokens"

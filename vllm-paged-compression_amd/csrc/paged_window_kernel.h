@@ -28,7 +28,9 @@
 
 namespace pe {
 
-constexpr float WIN_NEG = -1.0e30f;
+// below every finite score: the reference point of the weights before a visible key (f32's lowest number, not
+// -infinity, so that differences of two such points are 0)
+constexpr float WIN_NEG = -3.402823466e38f;
 constexpr int WIN_MAX_SPLITS = 32;
 
 // Conditions a launch survives (this translation unit's copy; read through pe_device_diagnostics)
@@ -299,6 +301,9 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   auto compute = [&](Tile& t, int tile) {
+    // A score is rounded once, before its maximum is taken and before that is subtracted: contracted into one
+    // multiply-add the subtraction would leave the rounding of the maximum, which is 2^8 for scores of 2^32.
+#pragma clang fp contract(off)
     const int t0 = tile * TOK;
     f32x4 s[NG];
 #pragma unroll
