@@ -104,3 +104,71 @@ def test_decode_window_scores_far_from_zero(ops, dtype, size, sign):
         ops.paged_attention_window(out, q[:1].cuda(), kc.cuda(), vc.cuda(), 1, D ** -0.5, t.cuda(), ln.cuda(), bs,
                                    max_len, 150, 2)
         assert torch.equal(out.cpu(), want.expand(1, 2, D)), f"launch shaped for {max_len} tokens"
+
+
+# ------------------------------------------------------------------ prefill scores far from zero
+@pytest.mark.parametrize("dtype,size", SIZES)
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window", [100, 300])
+def test_prefill_scores_far_from_zero(ops, dtype, size, sign, D, window):
+    """Rows that see one key far ahead of the others return its value; rows before it see equal scores and return
+    the mean of their values."""
+    g = torch.Generator().manual_seed(3)
+    n, ahead = 500, 150
+    q, k = far_scores(dtype, D, size, sign, n, ahead)
+    v = rows(g, n, 1, D, dtype)
+    # (one request takes the shape of launches that leave compute units idle, 40 take those of large ones)
+    for copies in (1, 40):
+        lens = [n] * copies
+        got = run_prefill(ops, *(x.repeat(copies, 1, 1) for x in (q, k, v)), lens, lens, window, 0, D ** -0.5).cpu()
+        for c in range(0, copies, 13):
+            one = got[c * n:(c + 1) * n]
+            assert torch.equal(one[ahead:ahead + window], v[ahead].expand(window, 2, D)), f"request {c} of {copies}"
+            mean = torch.stack([v[max(0, i - window + 1):i + 1].double().mean(0) for i in range(ahead)])
+            spread = torch.stack([v[max(0, i - window + 1):i + 1].double().abs().mean(0) for i in range(ahead)])
+            # equal weights: one rounding of the mean, and f32 sums of up to 100 products
+            u = plain.HALF_STEP[dtype]
+            plain.assert_within(one[:ahead], mean.expand(ahead, 2, D),
+                                (mean.abs() * u + spread * (200 * 2.0 ** -24)
+                                 + 2.0 ** -25 * (dtype == torch.float16)).expand(ahead, 2, D), f"request {c} of {copies}")
+
+
+@pytest.mark.parametrize("dtype,big", [(torch.float16, 6e4), (torch.bfloat16, 1e5), (torch.bfloat16, 1e12)])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(100, 0), (300, 5), (0, 0)])
+def test_prefill_scores_near_and_far_from_zero(ops, dtype, big, D, window, sinks):
+    """Keys far below the others (the first tile, every seventh key after it) and one far above: far keys have no
+    weight beside near ones, a row that sees far ones alone returns their mean."""
+    g = torch.Generator().manual_seed(5)
+    n, above = 420, 350
+    i = torch.arange(n)
+    low = (i < 70) | (i % 7 == 0)
+    q, k, v = rows(g, n, 2, D, dtype), rows(g, n, 1, D, dtype), rows(g, n, 1, D, dtype)
+    q[:, :, 0], k[:, :, 0] = big, 0.0
+    k[low] = 0.0
+    k[low, :, 0] = -big
+    k[above, :, 0] = big
+    see = i[None] <= i[:, None]
+    if window:
+        see &= (i[None] > i[:, None] - window) | (i[None] < sinks)
+    heaviest = torch.where(i == above, 2, torch.where(low, 0, 1))[None].expand(n, n).masked_fill(~see, -1)
+    see &= heaviest == heaviest.amax(1, keepdim=True)
+    # near keys: attend_one's terms with prefill_reference's two (both in 64 bits, over the keys that count)
+    qn, kn = q.double().clone(), k.double().clone()
+    qn[:, :, 0] = 0                                     # what the keys that count together differ by
+    s = torch.matmul(qn.transpose(0, 1), kn[:, 0].T.contiguous()) * D ** -0.5
+    size = (torch.matmul(qn.abs().transpose(0, 1), kn[:, 0].abs().T.contiguous()) * D ** -0.5 * see).amax(2, keepdim=True)
+    p = torch.softmax(s.masked_fill(~see, float("-inf")), 2)
+    vv, u = v[:, 0].double(), plain.HALF_STEP[dtype]
+    ref, spread = torch.matmul(p, vv).transpose(0, 1), torch.matmul(p, vv.abs())
+    rel = 2 * u + 2 * size * (D + 4) * 2.0 ** -24 + 4 * 2.0 ** -22 + 2 * n * 2.0 ** -24
+    bound = (spread * rel).transpose(0, 1) + ref.abs() * u
+    heavy = torch.matmul(see.double(), vv.abs())[:, None] / torch.exp(s.masked_fill(~see, float("-inf"))
+                                                                     - s.masked_fill(~see, float("-inf")).amax(2, keepdim=True)).sum(2).T[..., None]
+    bound = bound + heavy * (2.0 ** -120 if dtype == torch.bfloat16 else 2.0 ** -19) + 2.0 ** -25 * (dtype == torch.float16)
+    for copies in (1, 40):
+        lens = [n] * copies
+        got = run_prefill(ops, *(x.repeat(copies, 1, 1) for x in (q, k, v)), lens, lens, window, sinks, D ** -0.5).cpu()
+        for c in range(0, copies, 13):
+            plain.assert_within(got[c * n:(c + 1) * n], ref, bound, f"request {c} of {copies}")

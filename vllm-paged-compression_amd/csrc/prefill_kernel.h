@@ -160,6 +160,8 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   // adds the (storage-type rounded) probabilities of a query row over the fragment's 32 keys, in
   // every lane of the row's column - no vector adds per element, no cross-lane sum at the end,
   // and numerator and denominator use the same rounded weights.
+  // WIN: a row starts below every finite score (f32's lowest number)
+  constexpr float NEG = WIN ? -3.402823466e38f : PF_NEG;
   float m_run[NR];
   f32x4 acc_l[NR];
   f32x4 acc[DT][NR];
@@ -168,7 +170,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   for (int j = 0; j < 8; ++j) ones[j] = (T)1.0f;
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    m_run[n] = PF_NEG;
+    m_run[n] = NEG;
     acc_l[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -209,8 +211,10 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   uint32_t v_chunk16 = (uint32_t)(swz_off_v<D>(lrow, lslot) - lrow * (D * 2));
   if ((int)(k_chunk16 >> 4) >= hchunks) k_chunk16 = 0;
   if ((int)(v_chunk16 >> 4) >= hchunks) v_chunk16 = 0;
-  const uint32_t k_lane_off = (uint32_t)lrow * k_row_bytes + k_chunk16;
-  const uint32_t v_lane_off = (uint32_t)lrow * v_row_bytes + v_chunk16;
+  uint32_t k_lane_off = (uint32_t)lrow * k_row_bytes + k_chunk16;
+  uint32_t v_lane_off = (uint32_t)lrow * v_row_bytes + v_chunk16;
+  // (the multiply-add has a 64-bit result: opaque copies keep half of it alive through the tiles, not all)
+  if constexpr (WIN) asm volatile("" : "+v"(k_lane_off), "+v"(v_lane_off), "+v"(k_chunk16), "+v"(v_chunk16));
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem +
                         (uint32_t)wave * 1024u;
   // M0 carries the LDS destination of an LDS-DMA load and nothing else in this kernel (the
@@ -294,6 +298,41 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     }
   };
 
+  // The reference point of the exponentials only has to be NEAR the row's maximum: it moves
+  // (and the accumulators are rescaled) when some row of the wave outgrew it by more than
+  // 2^PF_LAZY_LOG2, so the weights stay below that factor and the rescale, frequent with a
+  // strict running maximum, becomes rare.  The normalised output does not depend on it.
+  //
+  // WIN, far: a weight's multiply-add subtracts the rounded point from an exact product, so all weights of a row
+  // carry 2^(the point's rounding): up to 2^1 at scores of 2^24, past the weights' range at 2^28 (f16) and 2^31
+  // (bf16).  A wave that has met scores of 2^24 rounds its scores before it subtracts.  (Costs 0.5 to 2 %: 8 x
+  // 1024, window 256: 67.6 -> 68.1 us, 4 x 8192, window 1024: 606 -> 616.)
+  bool far = false;
+  auto move_reference = [&](int n, float m_tile) {
+    if (__builtin_amdgcn_ballot_w64(m_tile > m_run[n] + PF_LAZY_LOG2) == 0) return;  // wave-uniform
+    const float m_new = fmaxf(m_run[n], m_tile);
+    const float alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+    m_run[n] = m_new;
+    acc_l[n] *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt][n] *= alpha;
+    if constexpr (WIN) far |= __builtin_amdgcn_ballot_w64(m_new > NEG && fabsf(m_new) > 16777216.f) != 0;
+  };
+  // the weights of row tile n are 2^(s * (what this returns) - m_ref)
+  auto weight_factor = [&](f32x4 (&s)[NS][NR], int n, float& m_ref) -> float {
+    m_ref = m_run[n];
+    if (!WIN || !far) return scale_log2e;
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma clang fp contract(off)
+        s[sub][n][r] = s[sub][n][r] * scale_log2e - m_ref;
+      }
+    m_ref = 0.f;
+    return 1.f;
+  };
+
   auto compute = [&](int tile, int buf, auto masked_tag) {
     constexpr bool MASKED = decltype(masked_tag)::value;
     const int n0 = tile * BN;
@@ -330,7 +369,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
     vec8 pf[NR][NS / 2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      float mx = PF_NEG;
+      float mx = WIN ? -INFINITY : PF_NEG;
       if constexpr (MASKED) {
         const int qrow = wrow0 + n * 16 + c;
         const int limit = min(qrow, lkv - 1) - n0 - 4 * g;  // last attended (sub*16 + r)
@@ -345,25 +384,14 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[sub][n][r]);
       mx = max_xor_16_32(mx);
-      // The reference point of the exponentials only has to be NEAR the row's maximum: it moves
-      // (and the accumulators are rescaled) when some row of the wave outgrew it by more than
-      // 2^PF_LAZY_LOG2, so the weights stay below that factor and the rescale, frequent with a
-      // strict running maximum, becomes rare.  The normalised output does not depend on it.
-      const float m_tile = mx * scale_log2e;
-      if (__builtin_amdgcn_ballot_w64(m_tile > m_run[n] + PF_LAZY_LOG2) != 0) {  // wave-uniform
-        const float m_new = fmaxf(m_run[n], m_tile);
-        const float alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
-        m_run[n] = m_new;
-        acc_l[n] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[dt][n] *= alpha;
-      }
-      const float m_new = m_run[n];
+      move_reference(n, mx * scale_log2e);
+      float m_ref;
+      const float factor = weight_factor(s, n, m_ref);
 #pragma unroll
       for (int sub = 0; sub < NS; ++sub) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], scale_log2e, -m_new));
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], factor, -m_ref));
           pf[n][sub >> 1][(sub & 1) * 4 + r] = (T)p;
         }
       }
@@ -434,21 +462,15 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[sub][n][r]);
         }
-      const float m_tile = max_xor_16_32(mx) * scale_log2e;
-      if (__builtin_amdgcn_ballot_w64(m_tile > m_run[n] + PF_LAZY_LOG2) != 0) {  // wave-uniform
-        const float m_new = fmaxf(m_run[n], m_tile);
-        const float alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
-        m_run[n] = m_new;
-        acc_l[n] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[dt][n] *= alpha;
-      }
+      move_reference(n, max_xor_16_32(mx) * scale_log2e);
+      float m_ref;
+      const float factor = weight_factor(s, n, m_ref);
 #pragma unroll
       for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           pf[n][sub >> 1][(sub & 1) * 4 + r] =
-              on[sub] ? (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], scale_log2e, -m_run[n])) : (T)0.f;
+              on[sub] ? (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], factor, -m_ref)) : (T)0.f;
     }
 #pragma unroll
     for (int k2 = 0; k2 < NS / 2; ++k2)
@@ -571,7 +593,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
       const int qrow = wrow0 + row;
       if (qrow >= lq) continue;
       constexpr int E = D / 64;
-      float qe[E], o[E], m = PF_NEG, l = 0.f;
+      float qe[E], o[E], m = NEG, l = 0.f;
 #pragma unroll
       for (int t = 0; t < E; ++t) {
         const int d = lane + 64 * t;
@@ -580,6 +602,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
       }
       const int last = min(qrow, lkv - 1), first = window > 0 ? max(0, qrow - window + 1) : 0;
       for (int j = sinks > 0 ? 0 : first; j <= last; ++j) {
+#pragma clang fp contract(off)
         if (j >= sinks && j < first) {
           j = first;
           if (j > last) break;
