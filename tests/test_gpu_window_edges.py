@@ -172,3 +172,19 @@ def test_prefill_scores_near_and_far_from_zero(ops, dtype, big, D, window, sinks
         got = run_prefill(ops, *(x.repeat(copies, 1, 1) for x in (q, k, v)), lens, lens, window, sinks, D ** -0.5).cpu()
         for c in range(0, copies, 13):
             plain.assert_within(got[c * n:(c + 1) * n], ref, bound, f"request {c} of {copies}")
+
+
+# ------------------------------------------------------------------ memory
+def test_out_of_memory_is_torchs_error(ops):
+    """A fresh output that the allocator refuses: the exception that servers catch, and the next call works."""
+    q, k = (torch.ones(1 << 16, h, 128, dtype=torch.float16, device="cuda") for h in (4, 1))
+    sums = cu(0, 40)
+    torch.cuda.empty_cache()
+    try:
+        torch.cuda.set_per_process_memory_fraction(1e-4)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            ops.prefill_window(q, k, k, sums, sums, 40, 0.1, 5)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    out = ops.prefill_window(q, k, k, sums, sums, 40, 0.1, 5)
+    assert (out[:40] == 1).all()

@@ -197,6 +197,12 @@ PyObject* guarded(const char* what, Py_ssize_t n, Py_ssize_t want, F&& body) {
     REQ(n == want, PyExc_TypeError, "%s: %zd arguments expected, got %zd", what, want, n);
     return body();
   } catch (const PyFail&) {
+  } catch (const c10::OutOfMemoryError& e) {  // (as torch's own allocations raise it)
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    if (type) PyErr_SetString(type, e.what_without_backtrace());
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
   } catch (const c10::Error& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception& e) {
