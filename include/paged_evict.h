@@ -664,7 +664,9 @@ int pe_swap_blocks(const void* src, void* dst, const int64_t* block_mapping_host
  * kv rows j <= min(i, Lkv-1) with sliding_window == 0, or j > i - sliding_window, or j < num_sinks; a
  * query that sees no row gets zeros.  bf16 / f16, head sizes 32, 64, 80, 96, 112, 120, 128, 192,
  * 256, scale > 0.  max_q_len sizes the grid: rows of a request past it are not computed.  num_q_rows /
- * num_kv_rows: rows that q (out) and k / v have; a request that cu_q or cu_kv places past them is cut.
+ * num_kv_rows: rows that q (out) and k / v have; a request that cu_q or cu_kv places past them is cut (k
+ * and v may be NULL when num_kv_rows is 0).  Rows of out that no request reaches are left as they are.
+ * max_q_len up to 2^22, and up to 65535 row blocks of a workgroup (64 rows each or more).
  * A NaN or an infinity in k or v reaches the queries that see its row, no other (such rows cost much
  * more time).
  * ---------------------------------------------------------------------------------- */
@@ -688,7 +690,8 @@ typedef enum { PE_KV_SAME = 0, PE_KV_FP8_E4M3 = 1, PE_KV_INT8 = 2 } pe_kv_format
 /* Appends rows to sequences of an 8-bit cache.  Sequence s takes rows cu_q[s] .. cu_q[s+1]-1 of
  * key/value [num_tokens, num_kv_heads, head_size] (cu_q == NULL: row s, the rows of a decode step)
  * at positions seq_lens[s] - rows .. seq_lens[s] - 1, i.e. seq_lens counts them already; a sequence
- * with no rows or with length 0 is skipped.  max_q_len sizes the grid.
+ * with no rows or with length 0 is skipped.  max_q_len sizes the grid: too small it costs time, 0 writes
+ * nothing.
  *   scale   s = max(s_old, 2^ceil(log2(max |x| / FMAX))) over the block's new rows (FMAX 448 or 127;
  *           at least 2^-100; 0 while all is 0), s_old = 0 when the call writes offset 0 of the block:
  *           a block begins anew there, whatever it held
@@ -710,7 +713,8 @@ int pe_reshape_and_cache_8bit(const void* key, const void* value, void* key_cach
  * sequence s stands at position seq_lens[s] - 1 and sees the keys j < seq_lens[s] with
  * sliding_window == 0, or j >= seq_lens[s] - sliding_window, or j < num_sinks; blocks that hold no
  * such key are not read.  out [num_seqs, num_heads, head_size] dense; nothing visible: zeros.
- * Any number of query heads per KV head.  Scales may be any finite f32 >= 0.
+ * Any number of query heads per KV head.  Scales may be any finite f32 >= 0; scores, and sums over the keys of
+ * weight * code * scale, are f32.
  *   workspace  device scratch of at least pe_paged_window_workspace_bytes(...) bytes, NULL when that
  *              is 0.  Calls that overlap on one workspace race on it. */
 int64_t pe_paged_window_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int head_size,

@@ -180,11 +180,16 @@ def test_out_of_memory_is_torchs_error(ops):
     q, k = (torch.ones(1 << 16, h, 128, dtype=torch.float16, device="cuda") for h in (4, 1))
     sums = cu(0, 40)
     torch.cuda.empty_cache()
+    held = []
     try:
         torch.cuda.set_per_process_memory_fraction(1e-4)
+        with pytest.raises(torch.cuda.OutOfMemoryError):    # what other tests' tensors leave free of their segments
+            while True:
+                held.append(torch.empty(1 << 25, dtype=torch.uint8, device="cuda"))
         with pytest.raises(torch.cuda.OutOfMemoryError):
             ops.prefill_window(q, k, k, sums, sums, 40, 0.1, 5)
     finally:
+        del held
         torch.cuda.set_per_process_memory_fraction(1.0)
     out = ops.prefill_window(q, k, k, sums, sums, 40, 0.1, 5)
     assert (out[:40] == 1).all()

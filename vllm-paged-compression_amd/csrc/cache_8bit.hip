@@ -13,9 +13,9 @@
 // and the codes of a value row's four tokens meet in one dword by two row swaps and four byte permutes;
 // the block goes through LDS in the cache's layout and is stored 16 bytes per lane.  The KV heads of a
 // block are dispatched side by side: their pieces of a token's row lie side by side.
-// Bound: HBM (2 bytes read, 1 written per element): 4 x 8192 rows of 8 x 128, int8, 39 us (4.7 TB/s, a
-// copy's rate); a decode step (one row per sequence) by the chain of dependent loads lengths -> rows /
-// table -> scale: 64 x 8 x 128, 4.6 us.
+// Bound: HBM (2 bytes read, 1 written per element): 4 x 8192 rows of 8 x 128, int8, 39 us a pass (4.7 TB/s, a
+// copy's rate; passes follow each other and share their start and end, a launch alone takes 43); a decode step (one row per sequence) by the chain of dependent loads lengths -> rows /
+// table -> scale: 64 x 8 x 128, 4.9 us.
 #include <type_traits>
 
 #include "kv8.h"
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(64 * w8_waves(D, BLK)) void cache8_write_kernel(
     if (whole) {
       for (int it = tid; it < D * BLK / 16; it += THREADS) {
         // (8 value rows are BLK / 2 pieces of 16 bytes.  Rows in and codes out pass the caches once: with the
-        //  non-temporal hint 42.5 us, without 44.7)
+        //  non-temporal hint 39.1 us, without 41.9)
         __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(k_img)[it], reinterpret_cast<u32x4*>(kb) + it);
         __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(v_img)[it + it / (BLK / 2)],
                                     reinterpret_cast<u32x4*>(vb) + it);

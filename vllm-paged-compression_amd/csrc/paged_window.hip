@@ -73,7 +73,7 @@ static WinShape window_shape(int num_seqs, int num_heads, int num_kv_heads, int 
     s.splits = (int)((tiles + s.waves - 1) / s.waves);
   } else if (wgs > 64 && tiles * head_size <= 56 * 128 && wgs * tiles * head_size <= 6000 * 128) {
     s.waves = wide;  // splits would not fill the chip evenly, or cost more than they give
-  } else if (wgs <= 128) {  // bound by bandwidth: a workgroup per CU
+  } else if (wgs <= 128) {  // bound by bandwidth: a workgroup per CU (below 8 workgroups WIN_MAX_SPLITS leaves CUs idle)
     s.splits = (int)(256 / wgs);
   } else {  // three splits on every second CU; tiles of 8 KiB and less want the waves of two
     s.splits = wgs <= 170 ? 3 : head_size <= 64 ? 2 : 1;

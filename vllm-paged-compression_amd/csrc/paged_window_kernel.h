@@ -14,7 +14,7 @@
 //     make one k-step of O^T += V^T.P^T whose slots are ordered so that P is used where it lies.
 //   V, 8 bits: lane (g, c) loads all 16 tokens (16 bytes) of row 16*dt + c of group g, and P goes to
 //     the lane group of its tokens by a 4x4 transpose of row swaps (8 per tile of 64 tokens).  With P
-//     left where it lies the loads are 4 bytes: 260 instead of 168 us on 945 MB.
+//     left where it lies the loads are 4 bytes: 260 instead of 168 us on 945 MB (replayed from a graph).
 // 8-bit codes are converted to the query's type exactly; K's scale multiplies the f32 scores, V's
 // scale the probabilities.
 //
@@ -111,7 +111,7 @@ __host__ __device__ inline WinRange win_range(int len, int window, int sinks) {
 // does it.  Its block lies in the last tile, which one wave owns: that wave encodes the row, puts it
 // (and, where the block's scale grows, the re-expressed older codes) into the tile's registers and into
 // the cache, and goes on with the attention.  No other wave of the launch touches the block.
-// 64 x 776 tokens in e4m3: 20.6 us with the row, 18.6 without (the write in a launch of its own: 4.6);
+// 64 x 776 tokens in e4m3: 20.6 us with the row, 18.6 without (the write in a launch of its own: 4.9);
 // 64 x 200: 11.3 and 8.6.  (Every lane encoding the chunks it holds: 21.8 and 13.6.)
 template <typename T, typename C, int D, int WAVES, int BLK, bool STEP>
 __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_window_kernel(const WinArgs a) {
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
   constexpr int KC = (CHUNKS + 3) / 4;        // chunks per lane and token
   constexpr int DT = (D + 15) / 16;
   constexpr int PB = BLK == 8 ? 2 : 1;        // blocks per group
-  // K/V loads of the throughput shape carry the non-temporal hint (945 MB: 168 against 187 us); the
+  // K/V loads of the throughput shape carry the non-temporal hint (945 MB, replayed from a graph: 168 against 187 us); the
   // latency shape serves launches of a few megabytes, which run faster with plain loads
   constexpr bool STREAM = WAVES < 8;
   static_assert(D % EPC == 0 && (BLK == 8 || BLK == 16 || BLK == 32), "head size / block size");
@@ -391,6 +391,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
 #pragma unroll
         for (int r = 0; r < 4; ++r) w[h][r] = shown(h, r) ? w[h][r] : 0.f;
     }
+    // The second matrix product takes its weights in the row type: one rounding of each, by at most 2^-8
+    // (bf16) or 2^-11 (f16) of it; their sum l_run is of the unrounded ones, in f32 like the statistics.
     vec8 pf[NG / 2];
 #pragma unroll
     for (int h = 0; h < NG; ++h)
@@ -492,7 +494,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
       char* kw = const_cast<char*>(kbase) + blk * blk_bytes;
       char* vw = const_cast<char*>(vbase) + blk * blk_bytes;
       const bool grew = __builtin_amdgcn_ballot_w64(kj.grew || vj.grew) != 0;  // wave-uniform
-      if (grew) {
+      if (__builtin_expect(grew, 0)) {  // (17 x 1028 of 4104 tokens, 8-token blocks: 11.3 us, without the hint 11.6)
         if (kj.grew)
           for (int it = lane; it < CHUNKS * o * 4; it += 64)
             reencode_word<C>(reinterpret_cast<uint32_t*>(kw + it / (o * 4) * (BLK * 16)) + it % (o * 4), kj.factor());
@@ -556,7 +558,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES > 8 ? WAVES / 4 : 2) void paged_w
   };
 
   // ---- the wave's tiles ------------------------------------------------------------------------
-  // (A second tile in flight gains nothing: 167.8 against 167.6 us on 945 MB, 21.5 against 20.3 on
+  // (A second tile in flight gains nothing, replayed from a graph: 167.8 against 167.6 us on 945 MB, 21.5 against 20.3 on
   // 64 x 776 tokens; the waves of a CU hold 128 KiB in flight as it is.  A tile number past the end
   // only names table entries, which load_ids keeps inside the row.)
   for (int i = i0; i < R.tiles; i += step) {

@@ -41,13 +41,15 @@ extern "C" int pe_prefill_window(void* out, const void* q, const void* k, const 
   const float sl2 = scale * 1.4426950408889634f;
   // Tile shape: 16 x NR query rows per wave, 4 waves (8 at the 256 pitch), BN keys per tile; the waves
   // take the query heads of a KV head side by side (hpw of them; fewer where the blocks of 16 * NR * waves / hpw
-  // rows would be more than the 65535 of a grid dimension).  Measured on MI355X (us per launch over
-  // three sets of inputs; NR x BN = 2 x 64 / 1 x 64 / 1 x 32; 32 query and 8 KV heads x 128, 4 sinks; none
-  // = no window):
-  //   8 x 1024 tokens, window 64: 59 / 71 / 48, 128: 64 / 75 / 57, 256: 73 / 88 / 74, 384: 79 / 98 / 83,
-  //   none: 94 / 116 / 109; 4 x 4096, window 64: 112 / 138 / 95, 256: 151 / 187 / 150, 512: 203 / 249 / 227,
-  //   none: 567 / 717 / 696; 1 x 512, window 64: 11.9 / 8.4 / 8.2, 256: 16.2 / 11.2 / 12.3, none: 17.7 / 12.8 / 16.0;
-  //   12 heads x 64, 8 x 1024, window 64: 24 / 18 / 18, 256: 31 / 22 / 24, none: 32 / 27 / 33.
+  // rows would be more than the 65535 of a grid dimension).  Measured on MI355X (us per pass, passes over
+  // three sets of inputs replayed from a graph; NR x BN = 2 x 64 / 1 x 64 / 1 x 32; 32 query and 8 KV heads x 128
+  // unless given, 4 sinks; none = no window):
+  //   8 x 1024 tokens, window 64: 58 / 67 / 46, 128: 63 / 74 / 54, 256: 73 / 86 / 68, 384: 79 / 96 / 79,
+  //   none: 91 / 112 / 100; 4 x 4096, window 64: 114 / 138 / 92, 256: 154 / 189 / 147, 512: 204 / 254 / 225,
+  //   none: 568 / 708 / 676; 1 x 512, window 64: 12.1 / 8.4 / 8.3, 256: 16.7 / 11.6 / 12.8, none: 18.1 / 13.0 / 16.4;
+  //   12 heads x 64, 8 x 1024, window 64: 25 / 17 / 18, 256: 30 / 21 / 24, none: 31 / 26 / 31; 1 x 8192, window 256:
+  //   34 / 26 / 29, 1024: 61 / 51 / 62; 32 / 8 heads x 64, 4 x 8192, window 256: 215 / 187 / 197, 1024: 433 / 405 / 467,
+  //   none: 1377 / 1364 / 1641.
   // So: head sizes up to 64, and launches that leave CUs idle, take the 1 x 64 shape (more and smaller
   // workgroups; at 64 elements a key costs half the LDS reads); rows that see few keys the 1 x 32 shape, whose
   // tiles waste less at the window's two ends; everything else 2 x 64, which reads each K/V fragment from
