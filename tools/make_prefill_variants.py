@@ -36,13 +36,13 @@ def variant(name, text):
         text = text.replace("      stage_wait();\n      __syncthreads();\n    }\n  };", "    }\n  };")
     if name == "nosoftmax":
         text = text.replace(
-            "const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], scale_log2e, -m_new));",
+            "const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], factor, -m_ref));",
             "const float p = s[sub][n][r];")
     if name == "novalu":
         # no max, no exp, no rescale: P is the raw S (wrong numbers, same MFMA / LDS work)
         text = text.replace("for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[sub][n][r]);", "for (int r = 0; r < 1; ++r) mx = fmaxf(mx, s[sub][n][r]);")
         text = text.replace(
-            "const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], scale_log2e, -m_new));",
+            "const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][n][r], factor, -m_ref));",
             "const float p = s[sub][n][r];")
         text = text.replace("if (__builtin_amdgcn_ballot_w64(m_new > m_run[n]) != 0) {", "if (m_new > 1e30f) {")
     if name in ("nopv", "nopv_novalu", "qkonly"):

@@ -25,8 +25,9 @@
 // its rows sees it, without mask code if all of them see all of it.  The waves of a workgroup take the same
 // rows of several query heads of a KV head, so that they see the same keys.  Bound: matrix and vector
 // instructions of a wave one after the other, as in the causal form, and at short windows the two partly
-// visible ends: 4 x 8192 tokens, 32 / 8 heads x 128, window 1024, 16 sinks: 604 us, 782 TFLOP/s (visible
-// pairs only); 8 x 1024, window 256: 67 us, 410 TFLOP/s, with the inputs read at 2.3 TB/s beside it.
+// visible ends: 4 x 8192 tokens, 32 / 8 heads x 128, window 1024, 16 sinks: 617 us a pass, 766 TFLOP/s (visible
+// pairs only); 8 x 1024, window 256: 70 us, 392 TFLOP/s, with the inputs read at 2.2 TB/s beside it (passes over
+// three sets of inputs, one after the other; a launch alone under the profiler takes 5 to 15 % longer).
 #pragma once
 #include "pe_common.h"
 
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
   // WIN, far: a weight's multiply-add subtracts the rounded point from an exact product, so all weights of a row
   // carry 2^(the point's rounding): up to 2^1 at scores of 2^24, past the weights' range at 2^28 (f16) and 2^31
   // (bf16).  A wave that has met scores of 2^24 rounds its scores before it subtracts.  (Costs 0.5 to 2 %: 8 x
-  // 1024, window 256: 67.6 -> 68.1 us, 4 x 8192, window 1024: 606 -> 616.)
+  // 1024, window 256: 67.6 -> 68.1 us, 4 x 8192, window 1024: 606 -> 616, both replayed from a graph.)
   bool far = false;
   auto move_reference = [&](int n, float m_tile) {
     if (__builtin_amdgcn_ballot_w64(m_tile > m_run[n] + PF_LAZY_LOG2) == 0) return;  // wave-uniform
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void prefill_mfma_kernel(
         }
         const int k0 = n0 + sub * 16;
         // (a group that every row of the wave sees in full needs no mask: 1 to 2 % on long prompts.  With one row
-        //  tile per wave the branch costs registers that spill: 70 against 67 us on 8 x 1024, window 256)
+        //  tile per wave the branch costs registers that spill: 4 % on 8 x 1024, window 256)
         if (NR == 1 || !(k0 + 15 <= min(wrow0, lkv - 1) && (window == 0 || k0 > row_last - window || k0 + 15 < sinks))) {
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
