@@ -33,6 +33,10 @@ def test_prefill_without_kv_rows(ops, D, window, sinks):
     got = ops.prefill_window(q, none, none, cu(0, 1, 70), cu(0, 0, 0), 69, 0.1, window, sinks, out)
     assert got is out and (out[:70] == 0).all()
     assert (out[70:] == 7).all(), "rows behind the last request were touched"
+    for _ in range(4):                                 # a fresh output is all zeros, whatever its memory held
+        dirty = torch.full_like(out, float("nan"))
+        del dirty
+        assert (ops.prefill_window(q, none, none, cu(0, 1, 70), cu(0, 0, 0), 69, 0.1, window, sinks) == 0).all()
     # (prefix sums that name rows which are not there are cut)
     out.fill_(7)
     ops.prefill_window(q, none, none, cu(0, 1, 70), cu(0, 5, 300), 69, 0.1, window, sinks, out)

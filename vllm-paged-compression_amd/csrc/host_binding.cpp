@@ -347,8 +347,9 @@ PyObject* prefill_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const int dev = device_of({&q, &k, &v, &cu_q, &cu_kv, out.defined() ? &out : nullptr});
     const bool any = q.size(0) > 0 && cu_q.size(0) > 1 && max_q > 0;
-    // (a fresh output is zero where no launch writes it at all)
-    if (!out.defined()) out = any ? at::empty({q.size(0), Hq, D}, q.options()) : at::zeros({q.size(0), Hq, D}, q.options());
+    // (a fresh output is zero where there is nothing to attend)
+    if (!out.defined())
+      out = any && k.size(0) > 0 ? at::empty({q.size(0), Hq, D}, q.options()) : at::zeros({q.size(0), Hq, D}, q.options());
     if (any) {  // (without kv rows too: the kernel writes the zeros of the requests' rows)
       launch(what, dev, [&](void* st) {
         return pe_prefill_window(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),

@@ -1057,7 +1057,7 @@ def prefill_window(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     sees none gets zeros.  query [Tq, Hq, D], key/value [Tkv, Hkv, D] bf16 or f16 (f32 is refused);
     ``scale`` > 0; cu_q/cu_kv int32 prefix sums; ``max_q_len`` = the longest request.  Rows of ``out`` that
     belong to no request, or lie past ``max_q_len`` in theirs, are not written; a fresh output holds
-    zeros if there is no request or ``max_q_len`` is 0, and anything in such rows otherwise."""
+    zeros there if there is no request, no kv row, or ``max_q_len`` is 0, and anything otherwise."""
     return (_lib._host or _lib.load_host()).prefill_window(
         query, key, value, cu_q, cu_kv, max_q_len, scale, sliding_window, num_sinks, out)
 
