@@ -14,8 +14,8 @@
 // the block goes through LDS in the cache's layout and is stored 16 bytes per lane.  The KV heads of a
 // block are dispatched side by side: their pieces of a token's row lie side by side.
 // Bound: HBM (2 bytes read, 1 written per element): 4 x 8192 rows of 8 x 128, int8, 39 us a pass (4.7 TB/s, a
-// copy's rate; passes follow each other and share their start and end, a launch alone takes 43); a decode step (one row per sequence) by the chain of dependent loads lengths -> rows /
-// table -> scale: 64 x 8 x 128, 4.9 us.
+// copy's rate; passes follow each other and share their start and end, a launch alone takes 43); a decode step
+// (one row per sequence) by the chain of dependent loads lengths -> rows / table -> scale: 64 x 8 x 128, 4.9 us.
 #include <type_traits>
 
 #include "kv8.h"
@@ -157,7 +157,8 @@ __global__ __launch_bounds__(64 * w8_waves(D, BLK)) void cache8_write_kernel(
           v[BLK / 4] = d1;
         }
       } else if (slot >= o0 && slot < o1 && c < CH) {
-        if (!kj.exact) kc = enc(kr[i], kj, std::false_type{});  // (only a block with older rows has a scale from elsewhere)
+        // (only a block with older rows has a scale from elsewhere)
+        if (!kj.exact) kc = enc(kr[i], kj, std::false_type{});
         if (!vj.exact) vc = enc(vr[i], vj, std::false_type{});
         *reinterpret_cast<u32x2*>(kb + k_at) = kc;
 #pragma unroll
